@@ -98,9 +98,9 @@ ABI_VERSION = 3   # == COIN_ABI_VERSION of include/coin_hip.h (tests/test_abi.py
 _lib = None
 
 
-def build(verbose: bool = False) -> str:
-    """Compile the HIP sources for gfx950 in-tree (``make -C coin_amd/csrc``)."""
-    cmd = ["make", "-C", CSRC_DIR, "-j4"]
+def build(verbose: bool = False, everything: bool = False) -> str:
+    """Compile the HIP sources for gfx950 in-tree (``make -C coin_amd/csrc``); ``everything``: also those that are up to date."""
+    cmd = ["make", "-C", CSRC_DIR, "-j8"] + (["-B"] if everything else [])
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:
         print(res.stdout)
