@@ -19,7 +19,7 @@ HEADER_PATH = os.path.abspath(os.path.join(_HERE, "..", "include", "coin_hip.h")
 
 COIN_F32, COIN_BF16 = 0, 1
 COIN_NCHW, COIN_NHWC = 0, 1
-ACT_NONE, ACT_LEAKY_RELU, ACT_RELU = 0, 1, 2
+ACT_NONE, ACT_LEAKY_RELU, ACT_RELU, ACT_GELU, ACT_QUICK_GELU, ACT_SILU = 0, 1, 2, 3, 4, 5
 
 _ERRORS = {-1: "COIN_EINVAL (bad argument)", -2: "COIN_ESHAPE (unsupported shape)", -3: "COIN_EALIGN (misaligned pointer / ld)"}
 
@@ -50,7 +50,7 @@ class EmaTensor(ctypes.Structure):
 
 
 _P, _I, _F, _L, _Z = c_void_p, c_int, c_float, c_int64, ctypes.c_size_t
-# name -> argtypes ; every entry point returns int.  Mirrors include/coin_hip.h one to one
+# name -> argtypes ; every entry point returns int, the *_workspace_bytes queries size_t.  Mirrors include/coin_hip.h one to one
 # (tests/test_abi.py parses the header and checks this table against it).
 SIGNATURES = {
     "coin_roi_align_fwd": [_P, _I, _I, _I, _I, _I, _P, _I, _I, _I, _F, _I, _I, _P, _I, _P],
@@ -91,9 +91,20 @@ SIGNATURES = {
     "coin_sgd_step": [_P, _I, _L, _F, _F, _F, _I, _P, _P],
     "coin_weight_dgrad_layout": [_P, _I, _I, _P],
     "coin_ema_update": [_P, _I, _L, _F, _P],
+    "coin_attention_workspace_bytes": [_I] * 8,
+    "coin_attention_fwd": [_P] * 11 + [_I] * 7 + [_F, _I, _P, _Z, _P],
+    "coin_attention_bwd": [_P] * 19 + [_I] * 7 + [_F, _I, _P, _Z, _P],
+    "coin_residual_norm_fwd": [_P, _P, _P, _L, _P, _P, _I, _F, _P, _P, _I, _F, _I, _F, _P, _P, _P, _L, _I, _I, _I, _I, _P],
+    "coin_residual_norm_bwd_workspace_bytes": [_L, _I],
+    "coin_residual_norm_bwd": [_P, _P, _P, _L, _P, _P, _I, _P, _I, _I, _F] + [_P] * 10 + [_L, _I, _I, _I, _I, _P, _Z, _P],
+    "coin_linear_workspace_bytes": [_L, _I, _I, _I, _I],
+    "coin_linear_fwd": [_P, _L, _P, _L, _P, _I, _I, _P, _L, _P, _L, _I, _P, _L, _L, _I, _I, _I, _P, _Z, _P],
+    "coin_linear_dz": [_P, _L, _I, _P, _L, _P, _L, _P, _I, _L, _I, _I, _P, _Z, _P],
+    "coin_linear_bwd": [_P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _I, _L, _I, _I, _I, _P, _Z, _P],
+    "coin_pad_rows": [_P, _L, _P, _L, _L, _I, _I, _P],
 }
 
-ABI_VERSION = 3   # == COIN_ABI_VERSION of include/coin_hip.h (tests/test_abi.py); lib() refuses any other library
+ABI_VERSION = 4   # == COIN_ABI_VERSION of include/coin_hip.h (tests/test_abi.py); lib() refuses any other library
 
 _lib = None
 
@@ -138,7 +149,7 @@ def lib() -> ctypes.CDLL:
     for name, argtypes in SIGNATURES.items():
         fn = getattr(l, name)
         fn.argtypes = argtypes
-        fn.restype = c_int
+        fn.restype = ctypes.c_size_t if name.endswith("_workspace_bytes") else c_int
     l.coin_nms_workspace_bytes.argtypes = [c_int, c_int]
     l.coin_nms_workspace_bytes.restype = ctypes.c_size_t
     l.coin_conv_gemm_stats_bytes.argtypes = [c_int, c_int]

@@ -1,0 +1,592 @@
+// Linear layer with its bias, activation and residual in the epilogue (coin_linear_fwd / _bwd), float32 and bfloat16:
+//
+//   z = x W^T + b,   y = residual + act(z);      dz = dy o act'(z),   dx = dz W,   dW = dz^T x,   db = sum_rows dz
+//
+// One matrix-product kernel serves the three products: an operand is read with the contraction along its rows (x and W of the forward,
+// dz of dx) or across them (W of dx, both of dW).  Tiles go to LDS by the range-checked LDS-DMA as they lie in memory; the fragments of a
+// tile whose contraction runs across the rows come out through the transposing LDS read (bfloat16) or column reads (float32), so no
+// operand is ever transposed in memory.
+//
+// The forward keeps act'(z) where a gradient will be asked for, in half precision for bfloat16 tensors: 2^-12 off at most, a sixteenth of
+// what rounding dz to bfloat16 costs, and within its range for every activation here (|act'| < 1.2).  dz is one pass over dy and act'
+// which takes the column sums of db along (partials per row block, added in order: no atomics).
+//
+// Few tiles and a long contraction (dW of a narrow layer, a product of few rows) are cut along the contraction; the float32 partial tiles
+// meet in a second launch, in order, which applies the same epilogue.
+#include "common.h"
+#include "mfma_tile.h"
+
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+struct LinArgs {
+  const void *A, *B;
+  int64_t lda, ldb;       // elements
+  int M, N, K;            // rows and columns of the output, contraction
+  void* C; int64_t ldc;
+  int c_f32;              // C (and the residual) are float32
+  const void* bias; int bias_f32;
+  const void* res; int64_t ldr;
+  void* slope; int64_t lds_;   // act'(z): half (bfloat16 operands) / float
+  int act, vec;           // vec: 16-byte accesses of C, residual and slope rows
+  int split; float* part; // K pieces: float32 partials [split][M][N]
+  int tiles_m, tiles_n;
+};
+
+__device__ __forceinline__ float sigmoid_of(float x) { return 1.f / (1.f + expf(-x)); }
+
+// act(z), and act'(z) where it is kept
+template <bool SLOPE>
+__device__ __forceinline__ float act_of(float z, int act, float& slope) {
+  slope = 1.f;
+  if (act == COIN_ACT_NONE) return z;
+  if (act == COIN_ACT_RELU) {
+    slope = z > 0.f ? 1.f : 0.f;
+    return z > 0.f ? z : (z != z ? z : 0.f);
+  }
+  if (act == COIN_ACT_GELU) {
+    const float cdf = 0.5f * erfcf(z * -0.70710678118654752f);
+    if (SLOPE) slope = cdf + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+    return z * cdf;
+  }
+  const float a = act == COIN_ACT_QUICK_GELU ? 1.702f : 1.f;   // z sigmoid(a z)
+  const float s = sigmoid_of(a * z);
+  if (SLOPE) slope = s * (1.f + a * z * (1.f - s));
+  return z * s;
+}
+
+// eight columns of one row through the epilogue: v holds the product
+template <typename T>
+__device__ __forceinline__ void finish8(const LinArgs& p, float (&v)[8], const float (&bias)[8], int64_t row, int col) {
+  const int left = p.N - col;
+  float sl[8], r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = 0.f;
+  if (p.res) {
+    if (p.vec) {
+      if (p.c_f32) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>((const float*)p.res + row * p.ldr + col);
+        const f32x4 b = *reinterpret_cast<const f32x4*>((const float*)p.res + row * p.ldr + col + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          r[i] = a[i];
+          r[4 + i] = b[i];
+        }
+      } else {
+        const bf16x8 a = *reinterpret_cast<const bf16x8*>((const bf16_t*)p.res + row * p.ldr + col);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = (float)a[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) r[i] = p.c_f32 ? ((const float*)p.res)[row * p.ldr + col + i] : (float)((const bf16_t*)p.res)[row * p.ldr + col + i];
+    }
+  }
+  if (p.slope) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = act_of<true>(v[i] + bias[i], p.act, sl[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = act_of<false>(v[i] + bias[i], p.act, sl[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] += r[i];
+  if (p.vec) {
+    if (p.c_f32) {
+      float* c = (float*)p.C + row * p.ldc + col;
+      *reinterpret_cast<f32x4*>(c) = (f32x4){v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4*>(c + 4) = (f32x4){v[4], v[5], v[6], v[7]};
+    } else {
+      bf16x8 o;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = (bf16_t)v[i];
+      *reinterpret_cast<bf16x8*>((bf16_t*)p.C + row * p.ldc + col) = o;
+    }
+    if (p.slope) {
+      if constexpr (sizeof(T) == 2) {
+        f16x8 o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = (_Float16)sl[i];
+        *reinterpret_cast<f16x8*>((_Float16*)p.slope + row * p.lds_ + col) = o;
+      } else {
+        float* c = (float*)p.slope + row * p.lds_ + col;
+        *reinterpret_cast<f32x4*>(c) = (f32x4){sl[0], sl[1], sl[2], sl[3]};
+        *reinterpret_cast<f32x4*>(c + 4) = (f32x4){sl[4], sl[5], sl[6], sl[7]};
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) {
+        if (p.c_f32) ((float*)p.C)[row * p.ldc + col + i] = v[i];
+        else ((bf16_t*)p.C)[row * p.ldc + col + i] = (bf16_t)v[i];
+        if (p.slope) {
+          if constexpr (sizeof(T) == 2) ((_Float16*)p.slope)[row * p.lds_ + col + i] = (_Float16)sl[i];
+          else ((float*)p.slope)[row * p.lds_ + col + i] = sl[i];
+        }
+      }
+  }
+}
+
+__device__ __forceinline__ void load_bias(const LinArgs& p, float (&b)[8], int col) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b[i] = p.bias && col + i < p.N ? (p.bias_f32 ? ((const float*)p.bias)[col + i] : (float)((const bf16_t*)p.bias)[col + i]) : 0.f;
+}
+
+// One operand of a tile: E rows (or columns) of the output, 128 bytes of the contraction.  ACROSS: the contraction runs across the rows
+template <typename T, bool ACROSS, int E, int NW>
+struct Operand {
+  static constexpr int EL = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T);
+  static constexpr int ROWB = ACROSS ? E * (int)sizeof(T) : 128, ROWS = ACROSS ? BK : E, BYTES = ROWS * ROWB;
+  // e0: first row of the tile (elements of the output), ext: how many there are; k0: first index of the contraction, K: its end
+  static __device__ __forceinline__ void stage(char* dst, const T* base, int64_t ld, int e0, int ext, int k0, int K, int wave, int lane) {
+    const unsigned st = (unsigned)(ld * sizeof(T));
+    if constexpr (ACROSS)
+      stage_tile<ROWB, ROWS, NW>(dst, base + (int64_t)k0 * ld + e0, K - k0, (ext - e0 + EL - 1) / EL, wave, lane, [&](int r) { return (unsigned)r * st; });
+    else
+      stage_tile<ROWB, ROWS, NW>(dst, base + (int64_t)e0 * ld + k0, ext - e0, (K - k0 + EL - 1) / EL, wave, lane, [&](int r) { return (unsigned)r * st; });
+  }
+  // fragment of the 32 rows from `row0`, step `s` of the contraction (32 bytes): lane & 31 = row, the lane half's 16 bytes
+  static __device__ __forceinline__ f32x4 frag_at(const char* img, int row0, int s, int lane) {
+    const int half = lane >> 5;
+    if constexpr (!ACROSS) {
+      return frag<128>(img, row0 + (lane & 31), 2 * s + half);
+    } else if constexpr (sizeof(T) == 2) {
+      const int q4 = (lane >> 2) & 3, p4 = lane & 3;
+      const int chunk = (row0 >> 3) + ((lane >> 4) & 1) * 2 + (p4 >> 1);
+      const int r0 = s * 16 + half * 8 + q4;
+      const char* a0 = img + r0 * ROWB + ((chunk ^ swz<ROWB>(r0)) << 4) + (p4 & 1) * 8;
+      const char* a1 = img + (r0 + 4) * ROWB + ((chunk ^ swz<ROWB>(r0 + 4)) << 4) + (p4 & 1) * 8;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a0);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a1);
+      const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      return __builtin_bit_cast(f32x4, v);
+    } else {
+      f32x4 v;
+      const int chunk = (row0 >> 2) + ((lane & 31) >> 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = s * 8 + half * 4 + e;
+        v[e] = *reinterpret_cast<const float*>(img + r * ROWB + ((chunk ^ swz<ROWB>(r)) << 4) + (lane & 3) * 4);
+      }
+      return v;
+    }
+  }
+};
+
+// C tile TS x TS by four waves (2 x 2), each (TS / 2)^2 in 32 x 32 accumulators; two stages of 128 contraction bytes per operand
+template <typename T, bool AA, bool BA, int TS>
+__global__ __launch_bounds__(256, 2) void linear_gemm_kernel(const LinArgs p) {
+  using OA = Operand<T, AA, TS, 4>;
+  using OB = Operand<T, BA, TS, 4>;
+  constexpr int BK = OA::BK, STAGE = OA::BYTES + OB::BYTES, W = TS / 64;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  static_assert(2 * STAGE >= TS * TS * 4, "the float32 epilogue image re-uses the ring");
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave >> 1, wc = wave & 1;
+  // XCD-aware order: workgroups b, b + 8, ... share an XCD and take neighbouring items of a contiguous eighth of the list; the list walks
+  // groups of 8 tile rows column by column, so what runs together shares 8 row panels and a few column panels in the XCD's L2
+  int item;
+  {
+    const int nwg = gridDim.x, q = nwg >> 3, r = nwg & 7, x = blockIdx.x & 7, i = blockIdx.x >> 3;
+    item = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + i;
+  }
+  const int piece = item % p.split, tile = item / p.split;
+  const int per = 8 * p.tiles_n, grp = tile / per, in = tile - grp * per;
+  const int gm = p.tiles_m - grp * 8 < 8 ? p.tiles_m - grp * 8 : 8;
+  const int tm = grp * 8 + in % gm, tn = in / gm;
+  const int m0 = tm * TS, n0 = tn * TS;
+  const int nk = (p.K + BK - 1) / BK;
+  const int kb = (int)((int64_t)piece * nk / p.split), ke = (int)((int64_t)(piece + 1) * nk / p.split);
+  auto stage = [&](int kt, int buf) {
+    char* d = lds + buf * STAGE;
+    OA::stage(d, (const T*)p.A, p.lda, m0, p.M, kt * BK, p.K, wave, lane);
+    OB::stage(d + OA::BYTES, (const T*)p.B, p.ldb, n0, p.N, kt * BK, p.K, wave, lane);
+  };
+  f32x16 acc[W][W];
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) acc[i][j] = zero16();
+  if (kb < ke) stage(kb, 0);
+  int buf = 0;
+  for (int kt = kb; kt < ke; ++kt, buf ^= 1) {
+    TILE_WAIT();
+    if (kt + 1 < ke) stage(kt + 1, buf ^ 1);
+    const char* la = lds + buf * STAGE;
+    const char* lb = la + OA::BYTES;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      f32x4 a[W], b[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) a[i] = OA::frag_at(la, wr * (TS / 2) + i * 32, s, lane);
+#pragma unroll
+      for (int j = 0; j < W; ++j) b[j] = OB::frag_at(lb, wc * (TS / 2) + j * 32, s, lane);
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) mma<T>(acc[i][j], b[j], a[i]);   // swapped: lane = output row, registers = 4 consecutive columns
+    }
+  }
+  P8_LDS_SYNC();   // every wave is done with the ring: it becomes the epilogue image [TS][TS] float32, 16-byte chunk c of row r at c ^ (r & 7)
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const int row = wr * (TS / 2) + i * 32 + (lane & 31);
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int ch = (wc * (TS / 2) + j * 32 + 2 * r + 4 * half) >> 2;
+        *reinterpret_cast<f32x4*>(lds + row * (TS * 4) + ((ch ^ (row & 7)) << 4)) = (f32x4){acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
+      }
+  }
+  P8_LDS_SYNC();
+  constexpr int TPR = TS / 8, RPP = 256 / TPR;
+  const int c8 = threadIdx.x % TPR, col = n0 + c8 * 8;
+  if (col >= p.N) return;
+  float bias[8];
+  if (p.split == 1) load_bias(p, bias, col);
+  for (int rr = threadIdx.x / TPR; rr < TS && m0 + rr < p.M; rr += RPP) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(lds + rr * (TS * 4) + (((2 * c8) ^ (rr & 7)) << 4));
+    const f32x4 y = *reinterpret_cast<const f32x4*>(lds + rr * (TS * 4) + (((2 * c8 + 1) ^ (rr & 7)) << 4));
+    if (p.split > 1) {
+      float* o = p.part + ((int64_t)piece * p.M + m0 + rr) * p.N + col;
+      if (p.N % 8 == 0) {
+        *reinterpret_cast<f32x4*>(o) = x;
+        *reinterpret_cast<f32x4*>(o + 4) = y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (col + i < p.N) o[i] = i < 4 ? x[i & 3] : y[i & 3];
+      }
+    } else {
+      float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      finish8<T>(p, v, bias, m0 + rr, col);
+    }
+  }
+}
+
+// the K pieces of eight columns of a row, in order, and the epilogue
+template <typename T>
+__global__ __launch_bounds__(256) void linear_join_kernel(const LinArgs p) {
+  const int n8 = (p.N + 7) / 8;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= (int64_t)p.M * n8) return;
+  const int64_t row = at / n8;
+  const int col = (int)(at - row * n8) * 8;
+  float v[8], bias[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  for (int s = 0; s < p.split; ++s) {
+    const float* o = p.part + ((int64_t)s * p.M + row) * p.N + col;
+    if (p.N % 8 == 0) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(o), y = *reinterpret_cast<const f32x4*>(o + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] += x[i];
+        v[4 + i] += y[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < p.N) v[i] += o[i];
+    }
+  }
+  load_bias(p, bias, col);
+  finish8<T>(p, v, bias, row, col);
+}
+
+// dz = dy o act' (rows of ldz elements, zeros behind N) and the column sums of dz per block of rows.  32 threads x 8 columns, 8 rows at a time
+struct DzArgs {
+  const void* dy; int64_t ldy; int dy_f32;
+  const void* slope; int64_t lds_;
+  void* dz; int64_t ldz;     // null: dz is dy itself, only its column sums are wanted
+  float* part;               // [row blocks][N] or null
+  int64_t M; int N, rows, vec;   // rows of a block; vec: 16-byte accesses of dy and slope rows
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void linear_dz_kernel(const DzArgs p) {
+  __shared__ float red[8][256];
+  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, col = (blockIdx.x * 32 + cx) * 8, left = p.N - col;
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = 0.f;
+  const int64_t r0 = (int64_t)blockIdx.y * p.rows, r1 = r0 + p.rows < p.M ? r0 + p.rows : p.M;
+  if (left > 0)
+    for (int64_t r = r0 + ry; r < r1; r += 8) {
+      float d[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d[i] = 0.f;
+      if (p.vec) {
+        if (p.dy_f32) {
+          const f32x4 a = *reinterpret_cast<const f32x4*>((const float*)p.dy + r * p.ldy + col);
+          const f32x4 b = *reinterpret_cast<const f32x4*>((const float*)p.dy + r * p.ldy + col + 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            d[i] = a[i];
+            d[4 + i] = b[i];
+          }
+        } else {
+          const bf16x8 a = *reinterpret_cast<const bf16x8*>((const bf16_t*)p.dy + r * p.ldy + col);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[i] = (float)a[i];
+        }
+        if (p.slope) {
+          if constexpr (sizeof(T) == 2) {
+            const f16x8 a = *reinterpret_cast<const f16x8*>((const _Float16*)p.slope + r * p.lds_ + col);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] *= (float)a[i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] *= ((const float*)p.slope)[r * p.lds_ + col + i];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < left) {
+            d[i] = p.dy_f32 ? ((const float*)p.dy)[r * p.ldy + col + i] : (float)((const bf16_t*)p.dy)[r * p.ldy + col + i];
+            if (p.slope) {
+              if constexpr (sizeof(T) == 2) d[i] *= (float)((const _Float16*)p.slope)[r * p.lds_ + col + i];
+              else d[i] *= ((const float*)p.slope)[r * p.lds_ + col + i];
+            }
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += d[i];
+      if (p.dz) {   // ldz is a multiple of 8 and covers whole chunks
+        if constexpr (sizeof(T) == 2) {
+          bf16x8 o;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = (bf16_t)d[i];
+          *reinterpret_cast<bf16x8*>((bf16_t*)p.dz + r * p.ldz + col) = o;
+        } else {
+          float* o = (float*)p.dz + r * p.ldz + col;
+          *reinterpret_cast<f32x4*>(o) = (f32x4){d[0], d[1], d[2], d[3]};
+          *reinterpret_cast<f32x4*>(o + 4) = (f32x4){d[4], d[5], d[6], d[7]};
+        }
+      }
+    }
+  if (!p.part) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) red[ry][cx * 8 + i] = s[i];
+  __syncthreads();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= p.N) return;
+  float t = red[0][threadIdx.x];
+#pragma unroll
+  for (int y = 1; y < 8; ++y) t += red[y][threadIdx.x];
+  p.part[(int64_t)blockIdx.y * p.N + c] = t;
+}
+
+// db: the row blocks' column sums, in order; 64 columns x 4 runs of blocks
+__global__ __launch_bounds__(256) void linear_db_kernel(const float* part, void* db, int db_f32, int blocks, int N) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, run = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+  const int per = (blocks + 3) / 4, b0 = run * per, b1 = b0 + per < blocks ? b0 + per : blocks;
+  float s = 0.f;
+  if (col < N)
+    for (int b = b0; b < b1; ++b) s += part[(int64_t)b * N + col];
+  red[run][lane] = s;
+  __syncthreads();
+  if (run || col >= N) return;
+  s = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
+  if (db_f32) ((float*)db)[col] = s;
+  else ((bf16_t*)db)[col] = (bf16_t)s;
+}
+
+// rows of `cols` elements -> rows of `ldd` elements, zeros behind the columns
+template <typename T>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const T* src, int64_t lds_, T* dst, int64_t ldd, int64_t rows, int cols) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, n8 = ldd / 8;
+  if (at >= rows * n8) return;
+  const int64_t r = at / n8;
+  const int c = (int)(at - r * n8) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) dst[r * ldd + c + i] = c + i < cols ? src[r * lds_ + c + i] : (T)0.f;
+}
+
+constexpr int64_t SPAN = 0x7fffffff;
+constexpr int CUS = 256;   // MI355X
+
+// Tile size and K pieces of one product.  128 x 128 tiles where they fill the chip, else 64 x 64; if even those are fewer than two
+// workgroups per CU, the contraction is cut so that they become that many, in pieces of at least four stages
+static void plan(int64_t M, int64_t N, int64_t K, int es, int* ts, int* split) {
+  const int64_t t128 = ((M + 127) / 128) * ((N + 127) / 128), nk = (K * es + 127) / 128;
+  *ts = t128 >= CUS ? 128 : 64;
+  const int64_t t = *ts == 128 ? t128 : ((M + 63) / 64) * ((N + 63) / 64);
+  int64_t s = t >= CUS ? 1 : 2 * CUS / t;
+  if (s > nk / 4) s = nk / 4;
+  if (s > 64) s = 64;
+  *split = s < 1 ? 1 : (int)s;
+}
+
+static size_t part_bytes(int64_t M, int64_t N, int64_t K, int es) {
+  int ts, s;
+  plan(M, N, K, es, &ts, &s);
+  return s > 1 ? (size_t)s * M * N * sizeof(float) : 0;
+}
+
+template <typename T, bool AA, bool BA>
+static void run_gemm(LinArgs a, hipStream_t st) {
+  int ts;
+  plan(a.M, a.N, a.K, sizeof(T), &ts, &a.split);
+  a.tiles_m = (a.M + ts - 1) / ts;
+  a.tiles_n = (a.N + ts - 1) / ts;
+  const unsigned grid = (unsigned)(a.tiles_m * a.tiles_n * a.split);
+  if (ts == 128) linear_gemm_kernel<T, AA, BA, 128><<<grid, 256, 0, st>>>(a);
+  else linear_gemm_kernel<T, AA, BA, 64><<<grid, 256, 0, st>>>(a);
+  if (a.split > 1) linear_join_kernel<T><<<(unsigned)(((int64_t)a.M * ((a.N + 7) / 8) + 255) / 256), 256, 0, st>>>(a);
+}
+
+static int dz_blocks(int64_t M, int N, int* rows) {
+  // about four workgroups per CU; at least 32 rows of a block, so that the column sums stay small beside the rows
+  const int64_t cols = (N + 255) / 256;
+  int64_t b = (4 * CUS + cols - 1) / cols;
+  if (b > (M + 31) / 32) b = (M + 31) / 32;
+  int64_t r = ((M + b - 1) / b + 7) / 8 * 8;
+  *rows = (int)r;
+  return (int)((M + r - 1) / r);
+}
+
+static bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+static int check_lin(int64_t M, int N, int K, int dtype) {
+  if (M < 0 || N <= 0 || K <= 0 || (dtype != COIN_F32 && dtype != COIN_BF16)) return COIN_EINVAL;
+  if (M > (1 << 30) || N > (1 << 24) || K > (1 << 24)) return COIN_ESHAPE;
+  const int es = dtype == COIN_BF16 ? 2 : 4;
+  int ts, s;
+  const int64_t dims[3][3] = {{M, N, K}, {M, K, N}, {N, K, M}};
+  for (auto& d : dims) {   // grids below 2^31
+    plan(d[0] > 0 ? d[0] : 1, d[1], d[2] > 0 ? d[2] : 1, es, &ts, &s);
+    if (((d[0] + 63) / 64) * ((d[1] + 63) / 64) * s >= SPAN || d[0] * ((d[1] + 7) / 8) / 256 >= SPAN - 1) return COIN_ESHAPE;
+  }
+  return COIN_OK;
+}
+
+// an operand: 16-byte rows (the last chunk of a row may be read whole: `cols` rounded up to chunks fits the row pitch), offsets of a tile below 2^31
+static int check_op(const void* p, int64_t ld, int64_t cols, int es) {
+  if (!p) return COIN_EINVAL;
+  const int el = 16 / es;
+  if (!al16(p) || ld % el || ld < (cols + el - 1) / el * el) return COIN_EALIGN;
+  if (ld >= SPAN || 130 * ld * es + cols * es + 4096 >= SPAN) return COIN_ESHAPE;
+  return COIN_OK;
+}
+
+static bool act_ok(int act) { return act == COIN_ACT_NONE || act == COIN_ACT_RELU || act == COIN_ACT_GELU || act == COIN_ACT_QUICK_GELU || act == COIN_ACT_SILU; }
+
+}  // namespace
+
+extern "C" int coin_pad_rows(const void* src, int64_t ld_src, void* dst, int64_t ld_dst, int64_t rows, int cols, int dtype, void* stream) {
+  if (!src || !dst || rows < 0 || cols <= 0 || ld_dst < cols || (dtype != COIN_F32 && dtype != COIN_BF16)) return COIN_EINVAL;
+  if (ld_dst % 8 || rows * (ld_dst / 8) / 256 >= SPAN - 1) return COIN_ESHAPE;
+  if (rows == 0) return COIN_OK;
+  const unsigned grid = (unsigned)((rows * (ld_dst / 8) + 255) / 256);
+  if (dtype == COIN_BF16) pad_rows_kernel<bf16_t><<<grid, 256, 0, (hipStream_t)stream>>>((const bf16_t*)src, ld_src, (bf16_t*)dst, ld_dst, rows, cols);
+  else pad_rows_kernel<float><<<grid, 256, 0, (hipStream_t)stream>>>((const float*)src, ld_src, (float*)dst, ld_dst, rows, cols);
+  return coin_launch_status();
+}
+
+extern "C" size_t coin_linear_workspace_bytes(int64_t M, int N, int K, int dtype, int backward) {
+  if (check_lin(M, N, K, dtype) != COIN_OK || M == 0) return 0;
+  const int es = dtype == COIN_BF16 ? 2 : 4;
+  if (!backward) return part_bytes(M, N, K, es);
+  size_t a = part_bytes(M, K, N, es), b = part_bytes(N, K, M, es);
+  int rows;
+  const size_t c = (size_t)dz_blocks(M, N, &rows) * N * sizeof(float);
+  if (b > a) a = b;
+  return a > c ? a : c;
+}
+
+extern "C" int coin_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int act, const void* residual,
+                               int64_t ldr, void* y, int64_t ldy, int y_dtype, void* slope, int64_t ld_slope, int64_t M, int N, int K, int dtype,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_lin(M, N, K, dtype);
+  if (rc != COIN_OK) return rc;
+  if (!act_ok(act) || (y_dtype != COIN_F32 && y_dtype != COIN_BF16) || (dtype == COIN_F32 && y_dtype != COIN_F32)) return COIN_EINVAL;
+  if (bias && bias_dtype != COIN_F32 && bias_dtype != COIN_BF16) return COIN_EINVAL;
+  if (M == 0) return COIN_OK;
+  const int es = dtype == COIN_BF16 ? 2 : 4;
+  if (!y || ldy < N || (residual && ldr < N) || (slope && ld_slope < N)) return COIN_EINVAL;
+  if ((rc = check_op(x, ldx, K, es)) != COIN_OK || (rc = check_op(w, ldw, K, es)) != COIN_OK) return rc;
+  const size_t need = part_bytes(M, N, K, es);
+  if (need && (!workspace || workspace_bytes < need)) return COIN_EINVAL;
+  if (!al16(workspace)) return COIN_EALIGN;
+  LinArgs a = {};
+  a.A = x; a.lda = ldx; a.B = w; a.ldb = ldw; a.M = (int)M; a.N = N; a.K = K; a.C = y; a.ldc = ldy; a.c_f32 = y_dtype == COIN_F32;
+  a.bias = bias; a.bias_f32 = bias_dtype == COIN_F32; a.res = residual; a.ldr = ldr; a.slope = slope; a.lds_ = ld_slope; a.act = act;
+  a.vec = N % 8 == 0 && ldy % 8 == 0 && al16(y) && (!residual || (ldr % 8 == 0 && al16(residual))) && (!slope || (ld_slope % 8 == 0 && al16(slope)));
+  a.part = (float*)workspace;
+  if (dtype == COIN_BF16) run_gemm<bf16_t, false, false>(a, (hipStream_t)stream);
+  else run_gemm<float, false, false>(a, (hipStream_t)stream);
+  return coin_launch_status();
+}
+
+extern "C" int coin_linear_dz(const void* dy, int64_t ldy, int dy_dtype, const void* slope, int64_t ld_slope, void* dz, int64_t ldz, void* db, int db_dtype,
+                              int64_t M, int N, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_lin(M, N, 1, dtype);
+  if (rc != COIN_OK) return rc;
+  if (!dy || (!dz && !db) || M == 0 || (dy_dtype != COIN_F32 && dy_dtype != COIN_BF16) || (dtype == COIN_F32 && dy_dtype != COIN_F32)) return COIN_EINVAL;
+  if (db && db_dtype != COIN_F32 && db_dtype != COIN_BF16) return COIN_EINVAL;
+  if (ldy < N || (slope && ld_slope < N)) return COIN_EINVAL;
+  if (dz && (!al16(dz) || ldz % 8 || ldz < (N + 7) / 8 * 8)) return COIN_EALIGN;
+  DzArgs a = {};
+  a.dy = dy; a.ldy = ldy; a.dy_f32 = dy_dtype == COIN_F32; a.slope = slope; a.lds_ = ld_slope; a.dz = dz; a.ldz = ldz; a.M = M; a.N = N;
+  a.vec = N % 8 == 0 && ldy % 8 == 0 && al16(dy) && (!slope || (ld_slope % 8 == 0 && al16(slope)));
+  const int blocks = dz_blocks(M, N, &a.rows);
+  if (db) {
+    if (!workspace || workspace_bytes < (size_t)blocks * N * sizeof(float)) return COIN_EINVAL;
+    a.part = (float*)workspace;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((N + 255) / 256, blocks);
+  if (dtype == COIN_BF16) linear_dz_kernel<bf16_t><<<grid, 256, 0, st>>>(a);
+  else linear_dz_kernel<float><<<grid, 256, 0, st>>>(a);
+  if (db) linear_db_kernel<<<(N + 63) / 64, 256, 0, st>>>(a.part, db, db_dtype == COIN_F32, blocks, N);
+  return coin_launch_status();
+}
+
+extern "C" int coin_linear_bwd(const void* dz, int64_t ldz, const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx, int64_t lddx, void* dw,
+                               int64_t lddw, int dw_dtype, int64_t M, int N, int K, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_lin(M, N, K, dtype);
+  if (rc != COIN_OK) return rc;
+  if ((!dx && !dw) || M == 0) return COIN_EINVAL;
+  if (dw && dw_dtype != COIN_F32 && (dw_dtype != COIN_BF16 || dtype == COIN_F32)) return COIN_EINVAL;
+  const int es = dtype == COIN_BF16 ? 2 : 4;
+  if ((rc = check_op(dz, ldz, N, es)) != COIN_OK) return rc;
+  if (workspace && !al16(workspace)) return COIN_EALIGN;
+  hipStream_t st = (hipStream_t)stream;
+  if (dx) {
+    if (lddx < K) return COIN_EINVAL;
+    if ((rc = check_op(w, ldw, K, es)) != COIN_OK) return rc;
+    const size_t need = part_bytes(M, K, N, es);
+    if (need && (!workspace || workspace_bytes < need)) return COIN_EINVAL;
+  }
+  if (dw) {
+    if (lddw < K) return COIN_EINVAL;
+    if ((rc = check_op(x, ldx, K, es)) != COIN_OK) return rc;
+    const size_t need = part_bytes(N, K, M, es);
+    if (need && (!workspace || workspace_bytes < need)) return COIN_EINVAL;
+  }
+  if (dx) {
+    LinArgs a = {};
+    a.A = dz; a.lda = ldz; a.B = w; a.ldb = ldw; a.M = (int)M; a.N = K; a.K = N; a.C = dx; a.ldc = lddx; a.c_f32 = dtype == COIN_F32;
+    a.vec = K % 8 == 0 && lddx % 8 == 0 && al16(dx);
+    a.part = (float*)workspace;
+    if (dtype == COIN_BF16) run_gemm<bf16_t, false, true>(a, st);
+    else run_gemm<float, false, true>(a, st);
+  }
+  if (dw) {
+    LinArgs a = {};
+    a.A = dz; a.lda = ldz; a.B = x; a.ldb = ldx; a.M = N; a.N = K; a.K = (int)M; a.C = dw; a.ldc = lddw; a.c_f32 = dw_dtype == COIN_F32;
+    a.vec = K % 8 == 0 && lddw % 8 == 0 && al16(dw);
+    a.part = (float*)workspace;
+    if (dtype == COIN_BF16) run_gemm<bf16_t, true, true>(a, st);
+    else run_gemm<float, true, true>(a, st);
+  }
+  return coin_launch_status();
+}

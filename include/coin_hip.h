@@ -31,12 +31,15 @@ extern "C" {
 
 /* Bumped whenever a prototype below changes (2: round 4's signature changes -- coin_sgd_step gate, coin_bn_* ReLU mask, coin_anchor_match
  * candidate sets, ... -- and round 5's additions; 3: round 6 -- coin_conv_gemm_stats_tile_rows, the tile height argument of
- * coin_conv_gemm_stats_finalize, COIN_BN_MAX_PARTS 768).  The Python binding refuses a library whose version differs (coin_amd/_lib.py). */
-#define COIN_ABI_VERSION 3
+ * coin_conv_gemm_stats_finalize, COIN_BN_MAX_PARTS 768; 4: the transformer-block entry points -- coin_attention_*, coin_residual_norm_*,
+ * coin_linear_*, coin_pad_rows).  The Python binding refuses a library whose version differs (coin_amd/_lib.py). */
+#define COIN_ABI_VERSION 4
 
 enum { COIN_F32 = 0, COIN_BF16 = 1 };
 enum { COIN_NCHW = 0, COIN_NHWC = 1 };
-enum { COIN_ACT_NONE = 0, COIN_ACT_LEAKY_RELU = 1, COIN_ACT_RELU = 2 };
+enum { COIN_ACT_NONE = 0, COIN_ACT_LEAKY_RELU = 1, COIN_ACT_RELU = 2,
+       /* coin_linear_fwd only: z Phi(z), z sigmoid(1.702 z), z sigmoid(z) */
+       COIN_ACT_GELU = 3, COIN_ACT_QUICK_GELU = 4, COIN_ACT_SILU = 5 };
 
 enum {
   COIN_OK = 0,
@@ -456,6 +459,72 @@ typedef struct coin_ema_tensor {
 
 int coin_ema_update(const coin_ema_tensor* table, int num_tensors, int64_t max_numel, float keep,
                     void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Transformer blocks (the CLIP text encoder, coin/modeling/text_encoder/clip_text.py:31-60; the Swin student).  `dtype` COIN_F32 or
+ * COIN_BF16 throughout; every sum is float32, no atomics, the same bits on every run.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Attention.  q [B][Lq][Hq][D], k and v [B][Lk][Hkv][D], out [B][Lq][Hq][D], Hkv | Hq: query head h reads key head h / (Hq / Hkv).
+ *   s_ij = scale q_i.k_j for j < n_b and, with `causal`, j <= i + n_b - Lq;  out_i = sum_j softmax_j(s_ij) v_j;  a query without a key
+ *   gives zeros and takes no gradient.
+ * n_b = key_lengths[b] (device, clamped to 0 .. Lk) or Lk where key_lengths is NULL; k and v behind it are not used, whatever they hold.
+ * *_strides: HOST arrays of three element strides (sequence, token, head); the last dimension is contiguous.  Pointers and strides are
+ * multiples of 16 bytes (COIN_EALIGN), strides may be 0; 66 tokens' span below 2^31 bytes, D <= 128 and a multiple of 8 (bf16) / 4 (f32)
+ * (COIN_ESHAPE); scale > 0.
+ * lse (float32 [B][Hkv][Lq * Hq / Hkv], or NULL when no backward follows): log2 of the row's sum of exp, +inf without a key.
+ * out_lo (bfloat16, contiguous like out, 16-byte aligned, or NULL when no backward follows; not used in float32): what rounding took from out.
+ * workspace: coin_attention_workspace_bytes (0: none), 16-byte aligned. */
+size_t coin_attention_workspace_bytes(int B, int Lq, int Lk, int Hq, int Hkv, int D, int dtype, int backward);
+int coin_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                       void* out, const int64_t* out_strides, void* out_lo, float* lse, const int* key_lengths, int B, int Lq, int Lk, int Hq, int Hkv,
+                       int D, int causal, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+/* dq, dk, dv are OVERWRITTEN (keys behind n_b: zeros); out, out_lo and lse are the forward's. */
+int coin_attention_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                       const void* out, const int64_t* out_strides, const void* out_lo, const void* dout, const int64_t* dout_strides,
+                       const float* lse, const int* key_lengths, void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                       const int64_t* dv_strides, int B, int Lq, int Lk, int Hq, int Hkv, int D, int causal, float scale, int dtype,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Residual add with the norm behind the branch, its gate and scale, and the norm before the next branch:
+ *   r = x + scale * gate o N_post(y),   h = N_pre(r),    N = LayerNorm, or RMSNorm where rms != 0
+ * x, r [M][D] of stream_dtype; y, h [M][D] of branch_dtype (float32 streams take both types of branch, bfloat16 streams bfloat16); gate
+ * [M / rows_per_gate][D] of gate_dtype, or NULL; weights and biases float32 [D] or NULL (1 and 0).  y NULL: h = N_pre(x), r is not
+ * written.  has_post / has_pre: which norms there are.  Contiguous rows, D <= 8192 (COIN_ESHAPE); any D and alignment (rows of 16-byte
+ * chunks are the fast ones).  stats float32 [M][4], 16-byte aligned, or NULL when no backward follows. */
+int coin_residual_norm_fwd(const void* x, const void* y, const void* gate, int64_t rows_per_gate, const float* post_weight, const float* post_bias,
+                           int has_post, float post_eps, const float* pre_weight, const float* pre_bias, int has_pre, float pre_eps, int rms,
+                           float scale, void* r, void* h, float* stats, int64_t M, int D, int stream_dtype, int branch_dtype, int gate_dtype,
+                           void* stream);
+/* Its backward from dr (stream_dtype, or NULL) and dh (branch_dtype, or NULL): dx (stream_dtype), dy (branch_dtype), dgate (gate_dtype)
+ * and the float32 weight and bias gradients, each OVERWRITTEN or NULL where it is not wanted.  M > 0.
+ * workspace (16-byte aligned): coin_residual_norm_bwd_workspace_bytes where a weight, bias or gate gradient is wanted. */
+size_t coin_residual_norm_bwd_workspace_bytes(int64_t M, int D);
+int coin_residual_norm_bwd(const void* x, const void* y, const void* gate, int64_t rows_per_gate, const float* post_weight, const float* post_bias,
+                           int has_post, const float* pre_weight, int has_pre, int rms, float scale, const float* stats, const void* dr,
+                           const void* dh, void* dx, void* dy, void* dgate, float* dpost_weight, float* dpost_bias, float* dpre_weight,
+                           float* dpre_bias, int64_t M, int D, int stream_dtype, int branch_dtype, int gate_dtype, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Linear layer y = residual + act(x W^T + bias): x [M][K], W [N][K] of `dtype`; y, residual [M][N] of y_dtype (float32 layers: float32);
+ * act NONE, RELU, GELU, QUICK_GELU or SILU.  slope (NULL when no backward follows): act'(z) [M][ld_slope], half precision for bfloat16
+ * layers, float32 for float32 ones.
+ * x and W rows: 16-byte aligned, leading dimensions of whole 16-byte chunks that hold the row's last chunk whole (COIN_EALIGN; coin_pad_rows
+ * makes such rows); where K is not a multiple of a chunk (8 bf16, 4 f32) the rest of the last chunk holds ZEROS.  The same for dz below.
+ * 130 rows' span below 2^31 bytes (COIN_ESHAPE).  workspace: coin_linear_workspace_bytes, 16-byte aligned. */
+size_t coin_linear_workspace_bytes(int64_t M, int N, int K, int dtype, int backward);
+int coin_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int act, const void* residual,
+                    int64_t ldr, void* y, int64_t ldy, int y_dtype, void* slope, int64_t ld_slope, int64_t M, int N, int K, int dtype,
+                    void* workspace, size_t workspace_bytes, void* stream);
+/* dz = dy o slope (slope NULL: dy) in `dtype`, rows of ldz elements (a multiple of 8) with zeros in the rest of the last chunk, and/or
+ * db = column sums of dz before its rounding.  dz or db may be NULL.  M > 0. */
+int coin_linear_dz(const void* dy, int64_t ldy, int dy_dtype, const void* slope, int64_t ld_slope, void* dz, int64_t ldz, void* db, int db_dtype,
+                   int64_t M, int N, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+/* dx [M][K] = dz W of `dtype` and / or dw [N][K] = dz^T x of dw_dtype (float32 layers: float32).  M > 0. */
+int coin_linear_bwd(const void* dz, int64_t ldz, const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx, int64_t lddx, void* dw,
+                    int64_t lddw, int dw_dtype, int64_t M, int N, int K, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+/* dst [rows][ld_dst] = src [rows][cols] (row pitch ld_src) with zeros behind the columns; ld_dst a multiple of 8. */
+int coin_pad_rows(const void* src, int64_t ld_src, void* dst, int64_t ld_dst, int64_t rows, int cols, int dtype, void* stream);
 
 #ifdef __cplusplus
 }
