@@ -34,10 +34,35 @@ struct LinArgs {
   int tiles_m, tiles_n;
 };
 
-__device__ __forceinline__ float sigmoid_of(float x) { return 1.f / (1.f + expf(-x)); }
+// Phi(z) and exp(-z^2 / 2).  bfloat16 layers: Abramowitz & Stegun 7.1.26 (erfc x = exp(-x^2) P(t), t = 1 / (1 + p x), absolute error
+// 1.5e-7), which shares its exponential with the slope: 18 instructions an element where the library's erfc and exp take 80, and those 80
+// were 0.25 ms of 0.93 ms on [16381 x 8192] outputs.
+template <typename T>
+__device__ __forceinline__ void normal_cdf(float z, float& cdf, float& bell) {
+  if constexpr (sizeof(T) == 4) {
+    cdf = 0.5f * erfcf(z * -0.70710678118654752f);
+    bell = expf(-0.5f * z * z);
+  } else {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+    float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    q = __builtin_fmaf(q, t, 1.421413741f);
+    q = __builtin_fmaf(q, t, -0.284496736f);
+    q = __builtin_fmaf(q, t, 0.254829592f);
+    bell = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+    q = 0.5f * q * t * bell;   // Phi(-|z|)
+    cdf = z < 0.f ? q : 1.f - q;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float sigmoid_of(float x) {
+  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-x));
+  else return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
+}
 
 // act(z), and act'(z) where it is kept
-template <bool SLOPE>
+template <typename T, bool SLOPE>
 __device__ __forceinline__ float act_of(float z, int act, float& slope) {
   slope = 1.f;
   if (act == COIN_ACT_NONE) return z;
@@ -46,12 +71,13 @@ __device__ __forceinline__ float act_of(float z, int act, float& slope) {
     return z > 0.f ? z : (z != z ? z : 0.f);
   }
   if (act == COIN_ACT_GELU) {
-    const float cdf = 0.5f * erfcf(z * -0.70710678118654752f);
-    if (SLOPE) slope = cdf + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+    float cdf, bell;
+    normal_cdf<T>(z, cdf, bell);
+    if (SLOPE) slope = __builtin_fmaf(z * 0.39894228040143268f, bell, cdf);
     return z * cdf;
   }
   const float a = act == COIN_ACT_QUICK_GELU ? 1.702f : 1.f;   // z sigmoid(a z)
-  const float s = sigmoid_of(a * z);
+  const float s = sigmoid_of<T>(a * z);
   if (SLOPE) slope = s * (1.f + a * z * (1.f - s));
   return z * s;
 }
@@ -86,10 +112,10 @@ __device__ __forceinline__ void finish8(const LinArgs& p, float (&v)[8], const f
   }
   if (p.slope) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_of<true>(v[i] + bias[i], p.act, sl[i]);
+    for (int i = 0; i < 8; ++i) v[i] = act_of<T, true>(v[i] + bias[i], p.act, sl[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_of<false>(v[i] + bias[i], p.act, sl[i]);
+    for (int i = 0; i < 8; ++i) v[i] = act_of<T, false>(v[i] + bias[i], p.act, sl[i]);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] += r[i];
@@ -135,11 +161,14 @@ __device__ __forceinline__ void load_bias(const LinArgs& p, float (&b)[8], int c
   for (int i = 0; i < 8; ++i) b[i] = p.bias && col + i < p.N ? (p.bias_f32 ? ((const float*)p.bias)[col + i] : (float)((const bf16_t*)p.bias)[col + i]) : 0.f;
 }
 
-// One operand of a tile: E rows (or columns) of the output, 128 bytes of the contraction.  ACROSS: the contraction runs across the rows
+constexpr int BKB = 64;   // bytes of the contraction in a stage
+constexpr int NST = 3;    // stages of the ring
+
+// One operand of a stage: E rows (or columns) of the output, BKB bytes of the contraction.  ACROSS: the contraction runs across the rows
 template <typename T, bool ACROSS, int E, int NW>
 struct Operand {
-  static constexpr int EL = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T);
-  static constexpr int ROWB = ACROSS ? E * (int)sizeof(T) : 128, ROWS = ACROSS ? BK : E, BYTES = ROWS * ROWB;
+  static constexpr int EL = 16 / (int)sizeof(T), BK = BKB / (int)sizeof(T);
+  static constexpr int ROWB = ACROSS ? E * (int)sizeof(T) : BKB, ROWS = ACROSS ? BK : E, BYTES = ROWS * ROWB;
   // e0: first row of the tile (elements of the output), ext: how many there are; k0: first index of the contraction, K: its end
   static __device__ __forceinline__ void stage(char* dst, const T* base, int64_t ld, int e0, int ext, int k0, int K, int wave, int lane) {
     const unsigned st = (unsigned)(ld * sizeof(T));
@@ -152,7 +181,7 @@ struct Operand {
   static __device__ __forceinline__ f32x4 frag_at(const char* img, int row0, int s, int lane) {
     const int half = lane >> 5;
     if constexpr (!ACROSS) {
-      return frag<128>(img, row0 + (lane & 31), 2 * s + half);
+      return frag<BKB>(img, row0 + (lane & 31), 2 * s + half);
     } else if constexpr (sizeof(T) == 2) {
       const int q4 = (lane >> 2) & 3, p4 = lane & 3;
       const int chunk = (row0 >> 3) + ((lane >> 4) & 1) * 2 + (p4 >> 1);
@@ -176,14 +205,26 @@ struct Operand {
   }
 };
 
-// C tile TS x TS by four waves (2 x 2), each (TS / 2)^2 in 32 x 32 accumulators; two stages of 128 contraction bytes per operand
-template <typename T, bool AA, bool BA, int TS>
+// all but the youngest stage's PER DMA instructions of this wave have landed, or all of them
+template <int PER>
+__device__ __forceinline__ void wait_stage(bool another) {
+  static_assert(PER == 2 || PER == 4 || PER == 6, "");
+  if (!another) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  else if (PER == 2) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)" ::: "memory");
+  else if (PER == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
+}
+
+// C tile TM x TN by four waves (2 x 2), each TM / 2 x TN / 2 in 32 x 32 accumulators; a ring of three stages, two in flight under the third.
+// 256 x 128: 72 KiB of LDS and 128 accumulator registers, two workgroups per CU: one's epilogue, prologue and barriers run under the
+// other's matrix instructions.
+template <typename T, bool AA, bool BA, int TM, int TN>
 __global__ __launch_bounds__(256, 2) void linear_gemm_kernel(const LinArgs p) {
-  using OA = Operand<T, AA, TS, 4>;
-  using OB = Operand<T, BA, TS, 4>;
-  constexpr int BK = OA::BK, STAGE = OA::BYTES + OB::BYTES, W = TS / 64;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-  static_assert(2 * STAGE >= TS * TS * 4, "the float32 epilogue image re-uses the ring");
+  using OA = Operand<T, AA, TM, 4>;
+  using OB = Operand<T, BA, TN, 4>;
+  constexpr int BK = OA::BK, STAGE = OA::BYTES + OB::BYTES, WM = TM / 64, WN = TN / 64, PER = STAGE / 4096;
+  constexpr int RING = NST * STAGE, PASS = TM * TN * 4 <= RING ? 1 : 2, IMG = TM * TN * 4 / PASS;   // passes and bytes of the epilogue image
+  __shared__ __attribute__((aligned(1024))) char lds[RING > IMG ? RING : IMG];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave >> 1, wc = wave & 1;
@@ -198,73 +239,83 @@ __global__ __launch_bounds__(256, 2) void linear_gemm_kernel(const LinArgs p) {
   const int per = 8 * p.tiles_n, grp = tile / per, in = tile - grp * per;
   const int gm = p.tiles_m - grp * 8 < 8 ? p.tiles_m - grp * 8 : 8;
   const int tm = grp * 8 + in % gm, tn = in / gm;
-  const int m0 = tm * TS, n0 = tn * TS;
+  const int m0 = tm * TM, n0 = tn * TN;
   const int nk = (p.K + BK - 1) / BK;
   const int kb = (int)((int64_t)piece * nk / p.split), ke = (int)((int64_t)(piece + 1) * nk / p.split);
-  auto stage = [&](int kt, int buf) {
-    char* d = lds + buf * STAGE;
+  auto stage = [&](int kt, int slot) {
+    char* d = lds + slot * STAGE;
     OA::stage(d, (const T*)p.A, p.lda, m0, p.M, kt * BK, p.K, wave, lane);
     OB::stage(d + OA::BYTES, (const T*)p.B, p.ldb, n0, p.N, kt * BK, p.K, wave, lane);
   };
-  f32x16 acc[W][W];
+  f32x16 acc[WM][WN];
 #pragma unroll
-  for (int i = 0; i < W; ++i)
+  for (int i = 0; i < WM; ++i)
 #pragma unroll
-    for (int j = 0; j < W; ++j) acc[i][j] = zero16();
+    for (int j = 0; j < WN; ++j) acc[i][j] = zero16();
   if (kb < ke) stage(kb, 0);
-  int buf = 0;
-  for (int kt = kb; kt < ke; ++kt, buf ^= 1) {
-    TILE_WAIT();
-    if (kt + 1 < ke) stage(kt + 1, buf ^ 1);
-    const char* la = lds + buf * STAGE;
+  if (kb + 1 < ke) stage(kb + 1, 1);
+  int slot = 0;
+  for (int kt = kb; kt < ke; ++kt) {
+    wait_stage<PER>(kt + 1 < ke);   // stage kt has landed
+    P8_BAR();                       // for every wave, and nobody reads the slot of stage kt - 1 any more
+    if (kt + 2 < ke) stage(kt + 2, slot == 0 ? 2 : slot - 1);
+    const char* la = lds + slot * STAGE;
     const char* lb = la + OA::BYTES;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      f32x4 a[W], b[W];
+    for (int s = 0; s < BKB / 32; ++s) {
+      f32x4 a[WM], b[WN];
 #pragma unroll
-      for (int i = 0; i < W; ++i) a[i] = OA::frag_at(la, wr * (TS / 2) + i * 32, s, lane);
+      for (int j = 0; j < WN; ++j) b[j] = OB::frag_at(lb, wc * (TN / 2) + j * 32, s, lane);
 #pragma unroll
-      for (int j = 0; j < W; ++j) b[j] = OB::frag_at(lb, wc * (TS / 2) + j * 32, s, lane);
+      for (int i = 0; i < WM; ++i) a[i] = OA::frag_at(la, wr * (TM / 2) + i * 32, s, lane);
 #pragma unroll
-      for (int i = 0; i < W; ++i)
+      for (int i = 0; i < WM; ++i)
 #pragma unroll
-        for (int j = 0; j < W; ++j) mma<T>(acc[i][j], b[j], a[i]);   // swapped: lane = output row, registers = 4 consecutive columns
+        for (int j = 0; j < WN; ++j) mma<T>(acc[i][j], b[j], a[i]);   // swapped: lane = output row, registers = 4 consecutive columns
     }
+    slot = slot == 2 ? 0 : slot + 1;
   }
-  P8_LDS_SYNC();   // every wave is done with the ring: it becomes the epilogue image [TS][TS] float32, 16-byte chunk c of row r at c ^ (r & 7)
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const int row = wr * (TS / 2) + i * 32 + (lane & 31);
-#pragma unroll
-    for (int j = 0; j < W; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int ch = (wc * (TS / 2) + j * 32 + 2 * r + 4 * half) >> 2;
-        *reinterpret_cast<f32x4*>(lds + row * (TS * 4) + ((ch ^ (row & 7)) << 4)) = (f32x4){acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
-      }
-  }
-  P8_LDS_SYNC();
-  constexpr int TPR = TS / 8, RPP = 256 / TPR;
+  // the ring becomes the epilogue image, TM / PASS rows of TN float32, 16-byte chunk c of row r at c ^ (r & 7)
+  constexpr int ROWS = TM / PASS, TPR = TN / 8, RPP = 256 / TPR;
   const int c8 = threadIdx.x % TPR, col = n0 + c8 * 8;
-  if (col >= p.N) return;
   float bias[8];
   if (p.split == 1) load_bias(p, bias, col);
-  for (int rr = threadIdx.x / TPR; rr < TS && m0 + rr < p.M; rr += RPP) {
-    const f32x4 x = *reinterpret_cast<const f32x4*>(lds + rr * (TS * 4) + (((2 * c8) ^ (rr & 7)) << 4));
-    const f32x4 y = *reinterpret_cast<const f32x4*>(lds + rr * (TS * 4) + (((2 * c8 + 1) ^ (rr & 7)) << 4));
-    if (p.split > 1) {
-      float* o = p.part + ((int64_t)piece * p.M + m0 + rr) * p.N + col;
-      if (p.N % 8 == 0) {
-        *reinterpret_cast<f32x4*>(o) = x;
-        *reinterpret_cast<f32x4*>(o + 4) = y;
-      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (col + i < p.N) o[i] = i < 4 ? x[i & 3] : y[i & 3];
+  for (int pass = 0; pass < PASS; ++pass) {
+    P8_LDS_SYNC();   // every wave is done with what the image overwrites
+    if (PASS == 1 || wr == pass) {
+#pragma unroll
+      for (int i = 0; i < WM; ++i) {
+        const int row = (PASS == 1 ? wr * (TM / 2) : 0) + i * 32 + (lane & 31);
+#pragma unroll
+        for (int j = 0; j < WN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; r += 4) {
+            const int ch = (wc * (TN / 2) + j * 32 + 2 * r + 4 * half) >> 2;
+            *reinterpret_cast<f32x4*>(lds + row * (TN * 4) + ((ch ^ (row & 7)) << 4)) = (f32x4){acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
+          }
       }
-    } else {
-      float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      finish8<T>(p, v, bias, m0 + rr, col);
+    }
+    P8_LDS_SYNC();
+    if (col >= p.N) continue;
+    const int mp = m0 + pass * ROWS;
+    for (int rr = threadIdx.x / TPR; rr < ROWS && mp + rr < p.M; rr += RPP) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(lds + rr * (TN * 4) + (((2 * c8) ^ (rr & 7)) << 4));
+      const f32x4 y = *reinterpret_cast<const f32x4*>(lds + rr * (TN * 4) + (((2 * c8 + 1) ^ (rr & 7)) << 4));
+      if (p.split > 1) {
+        float* o = p.part + ((int64_t)piece * p.M + mp + rr) * p.N + col;
+        if (p.N % 8 == 0) {
+          *reinterpret_cast<f32x4*>(o) = x;
+          *reinterpret_cast<f32x4*>(o + 4) = y;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col + i < p.N) o[i] = i < 4 ? x[i & 3] : y[i & 3];
+        }
+      } else {
+        float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        finish8<T>(p, v, bias, mp + rr, col);
+      }
     }
   }
 }
@@ -413,33 +464,40 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const T* src, int64_t lds
 constexpr int64_t SPAN = 0x7fffffff;
 constexpr int CUS = 256;   // MI355X
 
-// Tile size and K pieces of one product.  128 x 128 tiles where they fill the chip, else 64 x 64; if even those are fewer than two
-// workgroups per CU, the contraction is cut so that they become that many, in pieces of at least four stages
-static void plan(int64_t M, int64_t N, int64_t K, int es, int* ts, int* split) {
-  const int64_t t128 = ((M + 127) / 128) * ((N + 127) / 128), nk = (K * es + 127) / 128;
-  *ts = t128 >= CUS ? 128 : 64;
-  const int64_t t = *ts == 128 ? t128 : ((M + 63) / 64) * ((N + 63) / 64);
+struct Tiling {
+  int tm, tn, split;
+};
+
+// Tile size and K pieces of one product: the largest of 256 x 128, 128 x 128 and 64 x 64 tiles that still fills the chip (two workgroups
+// per CU of the first, one of the second); if even 64 x 64 tiles are fewer than the CUs, the contraction is cut so that they become two per
+// CU, in pieces of at least eight stages
+static Tiling plan(int64_t M, int64_t N, int64_t K, int es) {
+  const int64_t tn = (N + 127) / 128, nk = (K * es + BKB - 1) / BKB;
+  if ((M + 255) / 256 * tn >= 2 * CUS) return {256, 128, 1};
+  const bool big = (M + 127) / 128 * tn >= CUS;
+  const int64_t t = big ? (M + 127) / 128 * tn : ((M + 63) / 64) * ((N + 63) / 64);
   int64_t s = t >= CUS ? 1 : 2 * CUS / t;
-  if (s > nk / 4) s = nk / 4;
+  if (s > nk / 8) s = nk / 8;
   if (s > 64) s = 64;
-  *split = s < 1 ? 1 : (int)s;
+  if (s < 1) s = 1;
+  return {big ? 128 : 64, big ? 128 : 64, (int)s};
 }
 
 static size_t part_bytes(int64_t M, int64_t N, int64_t K, int es) {
-  int ts, s;
-  plan(M, N, K, es, &ts, &s);
+  const int s = plan(M, N, K, es).split;
   return s > 1 ? (size_t)s * M * N * sizeof(float) : 0;
 }
 
 template <typename T, bool AA, bool BA>
 static void run_gemm(LinArgs a, hipStream_t st) {
-  int ts;
-  plan(a.M, a.N, a.K, sizeof(T), &ts, &a.split);
-  a.tiles_m = (a.M + ts - 1) / ts;
-  a.tiles_n = (a.N + ts - 1) / ts;
+  const Tiling t = plan(a.M, a.N, a.K, sizeof(T));
+  a.split = t.split;
+  a.tiles_m = (a.M + t.tm - 1) / t.tm;
+  a.tiles_n = (a.N + t.tn - 1) / t.tn;
   const unsigned grid = (unsigned)(a.tiles_m * a.tiles_n * a.split);
-  if (ts == 128) linear_gemm_kernel<T, AA, BA, 128><<<grid, 256, 0, st>>>(a);
-  else linear_gemm_kernel<T, AA, BA, 64><<<grid, 256, 0, st>>>(a);
+  if (t.tm == 256) linear_gemm_kernel<T, AA, BA, 256, 128><<<grid, 256, 0, st>>>(a);
+  else if (t.tm == 128) linear_gemm_kernel<T, AA, BA, 128, 128><<<grid, 256, 0, st>>>(a);
+  else linear_gemm_kernel<T, AA, BA, 64, 64><<<grid, 256, 0, st>>>(a);
   if (a.split > 1) linear_join_kernel<T><<<(unsigned)(((int64_t)a.M * ((a.N + 7) / 8) + 255) / 256), 256, 0, st>>>(a);
 }
 
@@ -459,10 +517,9 @@ static int check_lin(int64_t M, int N, int K, int dtype) {
   if (M < 0 || N <= 0 || K <= 0 || (dtype != COIN_F32 && dtype != COIN_BF16)) return COIN_EINVAL;
   if (M > (1 << 30) || N > (1 << 24) || K > (1 << 24)) return COIN_ESHAPE;
   const int es = dtype == COIN_BF16 ? 2 : 4;
-  int ts, s;
   const int64_t dims[3][3] = {{M, N, K}, {M, K, N}, {N, K, M}};
   for (auto& d : dims) {   // grids below 2^31
-    plan(d[0] > 0 ? d[0] : 1, d[1], d[2] > 0 ? d[2] : 1, es, &ts, &s);
+    const int s = plan(d[0] > 0 ? d[0] : 1, d[1], d[2] > 0 ? d[2] : 1, es).split;
     if (((d[0] + 63) / 64) * ((d[1] + 63) / 64) * s >= SPAN || d[0] * ((d[1] + 7) / 8) / 256 >= SPAN - 1) return COIN_ESHAPE;
   }
   return COIN_OK;
@@ -473,7 +530,7 @@ static int check_op(const void* p, int64_t ld, int64_t cols, int es) {
   if (!p) return COIN_EINVAL;
   const int el = 16 / es;
   if (!al16(p) || ld % el || ld < (cols + el - 1) / el * el) return COIN_EALIGN;
-  if (ld >= SPAN || 130 * ld * es + cols * es + 4096 >= SPAN) return COIN_ESHAPE;
+  if (ld >= SPAN || 260 * ld * es + cols * es + 4096 >= SPAN) return COIN_ESHAPE;
   return COIN_OK;
 }
 

@@ -7,6 +7,7 @@ Nothing here computes on the CPU and nothing falls back to torch ops.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -17,7 +18,7 @@ from ._lib import ACT_LEAKY_RELU, ACT_NONE, ACT_RELU, COIN_BF16, COIN_F32, COIN_
 __all__ = [
     "roi_align_fwd", "roi_align_bwd", "gemm_nt", "conv_gemm", "conv_wgrad", "window_attn_fwd", "window_attn_bwd", "roi_align_fwd_levels", "roi_align_bwd_level", "conv_stats_finalize", "transpose2d", "bias_act_bwd", "cosine_logits_fwd",
     "cosine_logits_bwd", "bn_stats", "bn_apply_fwd", "bn_bwd", "avgpool2_fwd", "avgpool2_bwd", "nms_batched", "mil_ce", "mil_focal", "kl_div", "box_reg_l1", "l1_mean", "rpn_losses", "normalize_pad",
-    "SgdTable", "EmaTable", "attention_fwd", "attention_bwd", "residual_norm_fwd", "residual_norm_bwd", "chunked_rows", "linear_fwd", "linear_dz", "linear_bwd",
+    "SgdTable", "EmaTable", "attention_plan", "attention_fwd", "attention_bwd", "residual_norm_fwd", "residual_norm_bwd", "chunked_rows", "linear_fwd", "linear_dz", "linear_bwd",
 ]
 
 
@@ -958,170 +959,212 @@ class EmaTable:
 
 
 # --------------------------------------------------------------------------- transformer blocks
-class _on:
-    """The device of the operands is the current one inside (a launch goes to the current device's current stream)."""
+# A block's step is a handful of launches of a few microseconds each: what these wrappers do per call is kept small (addresses as plain
+# integers, what depends on shapes and strides alone computed once per shape).
+_WS_CACHE = 1024   # shapes whose workspace sizes are remembered
 
-    def __init__(self, *ts: Optional[torch.Tensor]):
-        _dev(*ts)
-        self.guard = None
-        index = None
-        for t in ts:
-            if t is None:
-                continue
-            i = t.get_device()
-            if index is None:
-                index = i
-            elif i != index:
-                raise CoinHipError("operands on different devices")
-        if index is not None and index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(index)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
+def _a(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
+
+def _device_of(*ts: Optional[torch.Tensor]) -> int:
+    """The one device index of the operands."""
+    index = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise CoinHipError("coin_amd kernels need device tensors (got a CPU tensor); there is no CPU path")
+        i = t.get_device()
+        if index is None:
+            index = i
+        elif i != index:
+            raise CoinHipError("operands on different devices")
+    return index
+
+
+def _launch(index: int, name: str, *args) -> None:
+    """Call an entry point on device `index` and its current stream."""
+    fn = getattr(_lib.lib(), name)
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _stream().value)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream().value)
+    if rc:
+        check(rc, name)
 
 
 def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-_I3 = ctypes.c_int64 * 3
-
-
 def _strides(t: torch.Tensor):
     """Element strides (sequence, token, head) for the C ABI; a dimension of size 1 has no stride of its own."""
-    return _I3(*[0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])])
+    return [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
 
 
-def _chunked(t: torch.Tensor) -> torch.Tensor:
-    """`t` [B, L, H, D] with whole 16-byte chunks along the last dimension: itself where pointer and strides allow it, else a copy."""
-    es = t.element_size()
-    if t.stride(3) == 1 and not t.data_ptr() & 15 and not any(n > 1 and (s * es) & 15 for n, s in zip(t.shape[:3], t.stride()[:3])):
-        return t
+def chunked_heads(t: torch.Tensor) -> torch.Tensor:
+    """`t` [..., D] with whole 16-byte chunks along the last dimension: itself where pointer and strides allow it, else a copy."""
+    if not t.data_ptr() & 15:
+        if t.is_contiguous() and (t.shape[-1] * t.element_size()) & 15 == 0:
+            return t
+        es = t.element_size()
+        if t.stride(-1) == 1 and not any(n > 1 and (s * es) & 15 for n, s in zip(t.shape[:-1], t.stride()[:-1])):
+            return t
     t = t.contiguous()
     return t.clone() if t.data_ptr() & 15 else t
 
 
-def _attention_dims(what: str, q, k, v, key_lengths, scale: float):
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
-        raise CoinHipError(f"{what}: q [B, Lq, Hq, D] and k, v [B, Lk, Hkv, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if q.dtype != k.dtype or q.dtype != v.dtype:
-        raise CoinHipError(f"{what}: q, k and v must share a dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
-    b, lq, hq, d = q.shape
-    lk, hkv = k.shape[1], k.shape[2]
-    if hkv == 0 or hq == 0 or hq % hkv:
-        raise CoinHipError(f"{what}: {hq} query heads over {hkv} key heads")
-    if d > 128 or d <= 0 or d % (16 // q.element_size()):
-        raise CoinHipError(f"{what}: head dimension {d} (a multiple of {16 // q.element_size()}, at most 128, for {q.dtype})")
+class AttentionPlan:
+    """What an attention call's shapes, strides and type decide: checked sizes, the strides of its eight tensors as the C ABI takes them (out
+    and the gradients contiguous, or the gradients strided like one [B, L, 3, H, D] tensor), workspace sizes."""
+    __slots__ = ("dims", "code", "strides", "at", "ws_fwd", "ws_bwd", "out_shape", "out_stride", "k_shape")
+
+    def __init__(self, q, k, v, packed: bool):
+        if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+            raise CoinHipError(f"attention: q [B, Lq, Hq, D] and k, v [B, Lk, Hkv, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+        if q.dtype != k.dtype or q.dtype != v.dtype:
+            raise CoinHipError(f"attention: q, k and v must share a dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+        self.code = _dt(q)
+        b, lq, hq, d = q.shape
+        lk, hkv = k.shape[1], k.shape[2]
+        if hkv == 0 or hq == 0 or hq % hkv:
+            raise CoinHipError(f"attention: {hq} query heads over {hkv} key heads")
+        if d > 128 or d <= 0 or d % (16 // q.element_size()):
+            raise CoinHipError(f"attention: head dimension {d} (a multiple of {16 // q.element_size()}, at most 128, for {q.dtype})")
+        self.dims = (b, lq, lk, hq, hkv, d)
+        self.out_shape, self.k_shape, self.out_stride = tuple(q.shape), tuple(k.shape), (lq * hq * d, hq * d, d, 1)
+        whole = [lq * hq * d, hq * d, d]
+        grads = [[3 * lq * hq * d, 3 * hq * d, d]] * 3 if packed else [whole] + [[lk * hkv * d, hkv * d, d]] * 2
+        rows = [_strides(q), _strides(k), _strides(v), whole, whole] + grads
+        self.strides = (ctypes.c_int64 * 24)(*sum(rows, []))
+        base = ctypes.addressof(self.strides)
+        self.at = [base + 24 * i for i in range(8)]   # q, k, v, out, dout, dq, dk, dv
+        ws = _lib.lib().coin_attention_workspace_bytes
+        self.ws_fwd, self.ws_bwd = (ws(b, lq, lk, hq, hkv, d, self.code, back) for back in (0, 1))
+
+
+_ATTN_PLANS: dict = {}
+
+
+def attention_plan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packed: bool = False) -> AttentionPlan:
+    key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, packed)
+    plan = _ATTN_PLANS.get(key)
+    if plan is None:
+        plan = AttentionPlan(q, k, v, packed)
+        if len(_ATTN_PLANS) >= 256:
+            _ATTN_PLANS.clear()
+        _ATTN_PLANS[key] = plan
+    return plan
+
+
+def attention_fwd(plan: AttentionPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scale: float,
+                  key_lengths: Optional[torch.Tensor] = None, keep: bool = False):
+    """coin_attention_fwd: q [B, Lq, Hq, D], k, v [B, Lk, Hkv, D] (`chunked_heads`) -> out [B, Lq, Hq, D] and, where a backward follows
+    (`keep`), log2 of the rows' sums and (bfloat16) what rounding took from out."""
+    b, lq, lk, hq, hkv, d = plan.dims
     if not 0.0 < scale < 3.0e38:
-        raise CoinHipError(f"{what}: scale must be positive and finite, got {scale}")
+        raise CoinHipError(f"attention: scale must be positive and finite, got {scale}")
     if key_lengths is not None and (key_lengths.dtype != torch.int32 or key_lengths.shape != (b,) or not key_lengths.is_contiguous()):
-        raise CoinHipError(f"{what}: key_lengths must be a contiguous int32 [{b}] tensor")
-    return b, lq, lk, hq, hkv, d
-
-
-def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scale: float, key_lengths: Optional[torch.Tensor] = None,
-                  keep: bool = False):
-    """coin_attention_fwd: q [B, Lq, Hq, D], k, v [B, Lk, Hkv, D] -> out [B, Lq, Hq, D] and, where a backward follows (`keep`), log2 of the
-    rows' sums and (bfloat16) what rounding took from out."""
-    dt = _dt(q)
-    b, lq, lk, hq, hkv, d = _attention_dims("attention_fwd", q, k, v, key_lengths, scale)
-    with _on(q, k, v, key_lengths):
-        out = torch.empty((b, lq, hq, d), dtype=q.dtype, device=q.device)
-        lse = torch.empty((b, hq * lq), dtype=torch.float32, device=q.device) if keep else None
-        lo = torch.empty_like(out) if keep and dt == COIN_BF16 else None
-        nbytes = _lib.lib().coin_attention_workspace_bytes(b, lq, lk, hq, hkv, d, dt, 0)
-        ws = _workspace(nbytes, q.device)
-        check(_lib.lib().coin_attention_fwd(_p(q), _strides(q), _p(k), _strides(k), _p(v), _strides(v), _p(out), _strides(out), _p(lo), _p(lse),
-                                            _p(key_lengths), b, lq, lk, hq, hkv, d, int(causal), float(scale), dt, _p(ws), nbytes, _stream()),
-              "coin_attention_fwd")
+        raise CoinHipError(f"attention: key_lengths must be a contiguous int32 [{b}] tensor")
+    index = _device_of(q, k, v, key_lengths)
+    dev = q.device
+    out = torch.empty(plan.out_shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(b * hq * lq, dtype=torch.float32, device=dev) if keep else None
+    lo = torch.empty(plan.out_shape, dtype=q.dtype, device=dev) if keep and plan.code == COIN_BF16 else None
+    ws = _workspace(plan.ws_fwd, dev)
+    at = plan.at
+    _launch(index, "coin_attention_fwd", q.data_ptr(), at[0], k.data_ptr(), at[1], v.data_ptr(), at[2], out.data_ptr(), at[3], _a(lo), _a(lse),
+            _a(key_lengths), b, lq, lk, hq, hkv, d, int(causal), scale, plan.code, _a(ws), plan.ws_fwd)
     return out, lse, lo
 
 
-def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lo: Optional[torch.Tensor], dout: torch.Tensor, lse: torch.Tensor,
-                  causal: bool, scale: float, key_lengths: Optional[torch.Tensor], dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor) -> None:
-    """coin_attention_bwd into dq, dk, dv (tensors of the operands' shapes, strided as `attention_fwd` takes them)."""
-    dt = _dt(q)
-    b, lq, lk, hq, hkv, d = _attention_dims("attention_bwd", q, k, v, key_lengths, scale)
-    if out.shape != q.shape or dout.shape != q.shape or dq.shape != q.shape or dk.shape != k.shape or dv.shape != k.shape or lse.numel() != b * hq * lq:
-        raise CoinHipError("attention_bwd: out, dout and dq are shaped like q, dk and dv like k")
-    if dt == COIN_BF16 and (lo is None or lo.shape != q.shape or lo.dtype != q.dtype or not lo.is_contiguous()):
-        raise CoinHipError("attention_bwd: the forward's residue of out is missing")
-    if any(t.dtype != q.dtype for t in (out, dout, dq, dk, dv)) or lse.dtype != torch.float32 or not lse.is_contiguous():
-        raise CoinHipError("attention_bwd: every tensor is of q's dtype, lse contiguous float32")
-    if any(t.stride(3) != 1 for t in (q, k, v, out, dout, dq, dk, dv) if t.numel()):
-        raise CoinHipError("attention_bwd: the last dimension must be contiguous")
-    with _on(q, k, v, out, lo, dout, lse, key_lengths, dq, dk, dv):
-        nbytes = _lib.lib().coin_attention_workspace_bytes(b, lq, lk, hq, hkv, d, dt, 1)
-        ws = _workspace(nbytes, q.device)
-        check(_lib.lib().coin_attention_bwd(_p(q), _strides(q), _p(k), _strides(k), _p(v), _strides(v), _p(out), _strides(out), _p(lo),
-                                            _p(dout), _strides(dout), _p(lse), _p(key_lengths), _p(dq), _strides(dq), _p(dk), _strides(dk), _p(dv),
-                                            _strides(dv), b, lq, lk, hq, hkv, d, int(causal), float(scale), dt, _p(ws), nbytes, _stream()),
-              "coin_attention_bwd")
+def attention_bwd(plan: AttentionPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lo: Optional[torch.Tensor], dout: torch.Tensor,
+                  lse: torch.Tensor, causal: bool, scale: float, key_lengths: Optional[torch.Tensor], dq: torch.Tensor, dk: torch.Tensor,
+                  dv: torch.Tensor) -> None:
+    """coin_attention_bwd into dq, dk, dv, laid out as the plan says, from `attention_fwd`'s results and dout (`chunked_heads`)."""
+    b, lq, lk, hq, hkv, d = plan.dims
+    if dout.shape != plan.out_shape or dout.dtype != q.dtype:
+        raise CoinHipError(f"attention: the gradient is {dout.dtype} {tuple(dout.shape)}, the output {q.dtype} {plan.out_shape}")
+    index = _device_of(q, k, v, out, dout, lse, key_lengths, dq, dk, dv)
+    ws = _workspace(plan.ws_bwd, q.device)
+    at, own = plan.at, None
+    dstrides = at[4]
+    if not dout.is_contiguous():
+        own = (ctypes.c_int64 * 3)(*_strides(dout))
+        dstrides = ctypes.addressof(own)
+    _launch(index, "coin_attention_bwd", q.data_ptr(), at[0], k.data_ptr(), at[1], v.data_ptr(), at[2], out.data_ptr(), at[3], _a(lo), dout.data_ptr(), dstrides,
+            lse.data_ptr(), _a(key_lengths), dq.data_ptr(), at[5], dk.data_ptr(), at[6], dv.data_ptr(), at[7], b, lq, lk, hq, hkv, d, int(causal), scale,
+            plan.code, _a(ws), plan.ws_bwd)
+
+
+def _code(dtype: torch.dtype) -> int:
+    return COIN_BF16 if dtype == torch.bfloat16 else COIN_F32
 
 
 def residual_norm_fwd(x: torch.Tensor, y: Optional[torch.Tensor], gate: Optional[torch.Tensor], rows_per_gate: int, post, pre, rms: bool, scale: float,
-                      branch_dtype: torch.dtype, want_stats: bool):
-    """coin_residual_norm_fwd on contiguous [M, D] rows; `post` / `pre` = (weight, bias, eps) or None -> (r or None, h or None, stats or None)."""
-    m, d = x.shape
+                      branch_dtype: torch.dtype, keep: bool):
+    """coin_residual_norm_fwd on contiguous [..., D] rows; `post` / `pre` = (weight, bias, eps) or None -> (r or None, h or None, and, where a
+    backward follows (`keep`), the rows' statistics)."""
+    d = x.shape[-1]
+    m = x.numel() // d
     pw, pb, peps = post if post is not None else (None, None, 0.0)
     nw, nb, neps = pre if pre is not None else (None, None, 0.0)
-    for t in (x, y, gate, pw, pb, nw, nb):
-        if t is not None and not t.is_contiguous():
-            raise CoinHipError("residual_norm_fwd needs contiguous operands")
-    with _on(x, y, gate, pw, pb, nw, nb):
-        r = torch.empty_like(x) if y is not None else None
-        h = torch.empty((m, d), dtype=branch_dtype, device=x.device) if pre is not None else None
-        stats = torch.empty((m, 4), dtype=torch.float32, device=x.device) if want_stats else None
-        bd = COIN_F32 if branch_dtype == torch.float32 else COIN_BF16
-        check(_lib.lib().coin_residual_norm_fwd(_p(x), _p(y), _p(gate), rows_per_gate, _p(pw), _p(pb), int(post is not None), float(peps), _p(nw), _p(nb),
-                                                int(pre is not None), float(neps), int(rms), float(scale), _p(r), _p(h), _p(stats), m, d, _dt(x), bd,
-                                                _dt(gate) if gate is not None else COIN_F32, _stream()), "coin_residual_norm_fwd")
+    index = _device_of(x, y, gate, pw, pb, nw, nb)
+    dev = x.device
+    r = torch.empty(x.shape, dtype=x.dtype, device=dev) if y is not None else None
+    h = torch.empty(x.shape, dtype=branch_dtype, device=dev) if pre is not None else None
+    stats = torch.empty((m, 4), dtype=torch.float32, device=dev) if keep else None
+    _launch(index, "coin_residual_norm_fwd", x.data_ptr(), _a(y), _a(gate), rows_per_gate, _a(pw), _a(pb), int(post is not None), peps, _a(nw), _a(nb),
+            int(pre is not None), neps, int(rms), scale, _a(r), _a(h), _a(stats), m, d, _code(x.dtype), _code(branch_dtype),
+            _code(gate.dtype) if gate is not None else COIN_F32)
     return r, h, stats
+
+
+@functools.lru_cache(_WS_CACHE)
+def _norm_ws(m: int, d: int) -> int:
+    return _lib.lib().coin_residual_norm_bwd_workspace_bytes(m, d)
 
 
 def residual_norm_bwd(x: torch.Tensor, y: Optional[torch.Tensor], gate: Optional[torch.Tensor], rows_per_gate: int, post, pre, rms: bool, scale: float,
                       stats: torch.Tensor, dr: Optional[torch.Tensor], dh: Optional[torch.Tensor], branch_dtype: torch.dtype, want):
     """coin_residual_norm_bwd; `want` = (dx, dy, dgate, dpost_weight, dpost_bias, dpre_weight, dpre_bias) truth values -> those gradients."""
-    m, d = x.shape
+    d = x.shape[-1]
+    m = x.numel() // d
     pw, pb, _ = post if post is not None else (None, None, 0.0)
     nw = pre[0] if pre is not None else None
-    with _on(x, y, gate, pw, pb, nw, stats, dr, dh):
-        f32 = lambda on: torch.empty(d, dtype=torch.float32, device=x.device) if on else None  # noqa: E731
-        dx = torch.empty_like(x) if want[0] else None
-        dy = torch.empty_like(y) if want[1] else None
-        dgate = torch.empty_like(gate) if want[2] else None
-        params = [f32(w) for w in want[3:]]
-        nbytes = _lib.lib().coin_residual_norm_bwd_workspace_bytes(m, d) if any(want[2:]) else 0
-        ws = _workspace(nbytes, x.device)
-        bd = COIN_F32 if branch_dtype == torch.float32 else COIN_BF16
-        check(_lib.lib().coin_residual_norm_bwd(_p(x), _p(y), _p(gate), rows_per_gate, _p(pw), _p(pb), int(post is not None), _p(nw),
-                                                int(pre is not None), int(rms), float(scale), _p(stats), _p(dr), _p(dh), _p(dx), _p(dy), _p(dgate),
-                                                *[_p(t) for t in params], m, d, _dt(x), bd, _dt(gate) if gate is not None else COIN_F32, _p(ws), nbytes,
-                                                _stream()), "coin_residual_norm_bwd")
+    index = _device_of(x, y, gate, pw, pb, nw, stats, dr, dh)
+    dev = x.device
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
+    dy = torch.empty(x.shape, dtype=y.dtype, device=dev) if want[1] else None
+    dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if want[2] else None
+    params = [torch.empty(d, dtype=torch.float32, device=dev) if w else None for w in want[3:]]
+    nbytes = _norm_ws(m, d) if any(want[2:]) else 0
+    ws = _workspace(nbytes, dev)
+    _launch(index, "coin_residual_norm_bwd", x.data_ptr(), _a(y), _a(gate), rows_per_gate, _a(pw), _a(pb), int(post is not None), _a(nw), int(pre is not None),
+            int(rms), scale, stats.data_ptr(), _a(dr), _a(dh), _a(dx), _a(dy), _a(dgate), *map(_a, params), m, d, _code(x.dtype), _code(branch_dtype),
+            _code(gate.dtype) if gate is not None else COIN_F32, _a(ws), nbytes)
     return (dx, dy, dgate, *params)
 
 
 def chunked_ok(x: torch.Tensor) -> bool:
     m, k = x.shape
     el = 16 // x.element_size()
-    return k % el == 0 and x.stride(1) == 1 and (m == 1 or (x.stride(0) % el == 0 and x.stride(0) >= k)) and not x.data_ptr() & 15
+    s0, s1 = x.stride()
+    return k % el == 0 and s1 == 1 and (m == 1 or (s0 % el == 0 and s0 >= k)) and not x.data_ptr() & 15
 
 
 def chunked_rows(x: torch.Tensor) -> torch.Tensor:
     """`x` [M, K] as rows of whole 16-byte chunks: itself where its pointer, pitch and K allow it, else a copy whose rows end in zeros."""
-    m, k = x.shape
     if chunked_ok(x):
         return x
+    m, k = x.shape
     if x.stride(1) != 1:
         x = x.contiguous()
     out = torch.empty((m, (k + 7) // 8 * 8), dtype=x.dtype, device=x.device)
-    with _on(x):
-        check(_lib.lib().coin_pad_rows(_p(x), x.stride(0), _p(out), out.stride(0), m, k, _dt(x), _stream()), "coin_pad_rows")
+    _launch(_device_of(x), "coin_pad_rows", x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0), m, k, _dt(x))
     return out
 
 
@@ -1131,48 +1174,50 @@ def _pitch(x: Optional[torch.Tensor]) -> int:
     return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), (x.shape[1] + 7) // 8 * 8)
 
 
+@functools.lru_cache(_WS_CACHE)
+def _linear_ws(m: int, n: int, k: int, code: int, backward: int) -> int:
+    return _lib.lib().coin_linear_workspace_bytes(m, n, k, code, backward)
+
+
 def linear_fwd(x: torch.Tensor, w: torch.Tensor, k: int, bias: Optional[torch.Tensor], act: int, residual: Optional[torch.Tensor], y_dtype: torch.dtype,
-               want_slope: bool):
-    """coin_linear_fwd on `chunked_rows` operands (k: the layer's own input width) -> y [M, N], act'(z) rows or None."""
+               keep: bool):
+    """coin_linear_fwd on `chunked_rows` operands (k: the layer's own input width) -> y [M, N] and, where a backward follows (`keep`), the
+    rows of act'(z)."""
     m, n = x.shape[0], w.shape[0]
-    with _on(x, w, bias, residual):
-        y = torch.empty((m, n), dtype=y_dtype, device=x.device)
-        slope = None
-        if want_slope:
-            slope = torch.empty((m, (n + 7) // 8 * 8), dtype=torch.float16 if x.dtype == torch.bfloat16 else torch.float32, device=x.device)
-        nbytes = _lib.lib().coin_linear_workspace_bytes(m, n, k, _dt(x), 0)
-        ws = _workspace(nbytes, x.device)
-        check(_lib.lib().coin_linear_fwd(_p(x), _pitch(x), _p(w), _pitch(w), _p(bias), _dt(bias) if bias is not None else COIN_F32, act, _p(residual),
-                                         _pitch(residual), _p(y), n, _dt(y), _p(slope),
-                                         slope.shape[1] if slope is not None else 0, m, n, k, _dt(x), _p(ws), nbytes, _stream()), "coin_linear_fwd")
+    index = _device_of(x, w, bias, residual)
+    dev, code = x.device, _code(x.dtype)
+    y = torch.empty((m, n), dtype=y_dtype, device=dev)
+    slope = torch.empty((m, (n + 7) // 8 * 8), dtype=torch.float16 if code == COIN_BF16 else torch.float32, device=dev) if keep else None
+    nbytes = _linear_ws(m, n, k, code, 0)
+    ws = _workspace(nbytes, dev)
+    _launch(index, "coin_linear_fwd", x.data_ptr(), _pitch(x), w.data_ptr(), _pitch(w), _a(bias), _code(bias.dtype) if bias is not None else COIN_F32, act,
+            _a(residual), _pitch(residual), y.data_ptr(), n, _code(y_dtype), _a(slope), slope.shape[1] if keep else 0, m, n, k, code, _a(ws), nbytes)
     return y, slope
 
 
 def linear_dz(dy: torch.Tensor, slope: Optional[torch.Tensor], dtype: torch.dtype, want_dz: bool, db_dtype: Optional[torch.dtype]):
     """coin_linear_dz: dz = dy o slope as rows for `linear_bwd`, and its column sums -> (dz or None, db or None)."""
     m, n = dy.shape
-    if dy.stride(1) != 1:
-        dy = dy.contiguous()
-    with _on(dy, slope):
-        dz = torch.empty((m, (n + 7) // 8 * 8), dtype=dtype, device=dy.device) if want_dz else None
-        db = torch.empty(n, dtype=db_dtype, device=dy.device) if db_dtype is not None else None
-        code = COIN_BF16 if dtype == torch.bfloat16 else COIN_F32
-        nbytes = _lib.lib().coin_linear_workspace_bytes(m, n, 1, code, 1) if db is not None else 0
-        ws = _workspace(nbytes, dy.device)
-        check(_lib.lib().coin_linear_dz(_p(dy), _pitch(dy), _dt(dy), _p(slope), slope.shape[1] if slope is not None else 0, _p(dz),
-                                        dz.shape[1] if dz is not None else 0, _p(db), _dt(db) if db is not None else COIN_F32, m, n, code, _p(ws), nbytes,
-                                        _stream()), "coin_linear_dz")
+    index = _device_of(dy, slope)
+    dev, code = dy.device, _code(dtype)
+    dz = torch.empty((m, (n + 7) // 8 * 8), dtype=dtype, device=dev) if want_dz else None
+    db = torch.empty(n, dtype=db_dtype, device=dev) if db_dtype is not None else None
+    nbytes = _linear_ws(m, n, 1, code, 1) if db is not None else 0
+    ws = _workspace(nbytes, dev)
+    _launch(index, "coin_linear_dz", dy.data_ptr(), _pitch(dy), _code(dy.dtype), _a(slope), slope.shape[1] if slope is not None else 0, _a(dz),
+            dz.shape[1] if want_dz else 0, _a(db), _code(db_dtype) if db is not None else COIN_F32, m, n, code, _a(ws), nbytes)
     return dz, db
 
 
 def linear_bwd(dz: torch.Tensor, x: Optional[torch.Tensor], w: Optional[torch.Tensor], n: int, k: int, want_dx: bool, dw_dtype: Optional[torch.dtype]):
     """coin_linear_bwd on `chunked_rows` operands -> (dx [M, k] or None, dW [n, k] or None); x serves dW, w serves dx."""
     m = dz.shape[0]
-    with _on(dz, x, w):
-        dx = torch.empty((m, k), dtype=dz.dtype, device=dz.device) if want_dx else None
-        dw = torch.empty((n, k), dtype=dw_dtype, device=dz.device) if dw_dtype is not None else None
-        nbytes = _lib.lib().coin_linear_workspace_bytes(m, n, k, _dt(dz), 1)
-        ws = _workspace(nbytes, dz.device)
-        check(_lib.lib().coin_linear_bwd(_p(dz), _pitch(dz), _p(x), _pitch(x), _p(w), _pitch(w), _p(dx), k, _p(dw), k,
-                                         _dt(dw) if dw is not None else COIN_F32, m, n, k, _dt(dz), _p(ws), nbytes, _stream()), "coin_linear_bwd")
+    index = _device_of(dz, x, w)
+    dev, code = dz.device, _code(dz.dtype)
+    dx = torch.empty((m, k), dtype=dz.dtype, device=dev) if want_dx else None
+    dw = torch.empty((n, k), dtype=dw_dtype, device=dev) if dw_dtype is not None else None
+    nbytes = _linear_ws(m, n, k, code, 1)
+    ws = _workspace(nbytes, dev)
+    _launch(index, "coin_linear_bwd", dz.data_ptr(), _pitch(dz), _a(x), _pitch(x), _a(w), _pitch(w), _a(dx), k, _a(dw), k,
+            _code(dw_dtype) if dw is not None else COIN_F32, m, n, k, code, _a(ws), nbytes)
     return dx, dw

@@ -889,30 +889,31 @@ def _wants_grad(*ts: Optional[torch.Tensor]) -> bool:
 
 class _Attention(Function):
     @staticmethod
-    def forward(ctx, q, k, v, key_lengths, causal, scale):
-        out, lse, lo = K.attention_fwd(q, k, v, causal, scale, key_lengths, keep=True)
+    def forward(ctx, q, k, v, key_lengths, causal, scale, plan):
+        out, lse, lo = K.attention_fwd(plan, q, k, v, causal, scale, key_lengths, keep=True)
         ctx.save_for_backward(q, k, v, out, lo, lse, key_lengths)
-        ctx.causal, ctx.scale = causal, scale
+        ctx.causal, ctx.scale, ctx.plan = causal, scale, plan
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lo, lse, lengths = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        K.attention_bwd(q, k, v, out, lo, K._chunked(dout.to(q.dtype)), lse, ctx.causal, ctx.scale, lengths, dq, dk, dv)
-        return dq, dk, dv, None, None, None
+        plan, dt, dev = ctx.plan, q.dtype, q.device
+        dq, dk, dv = (torch.empty(s, dtype=dt, device=dev) for s in (plan.out_shape, plan.k_shape, plan.k_shape))
+        K.attention_bwd(plan, q, k, v, out, lo, K.chunked_heads(dout), lse, ctx.causal, ctx.scale, lengths, dq, dk, dv)
+        return dq, dk, dv, None, None, None, None
 
 
 class _AttentionQKV(Function):
     """The same on one [B, L, 3, H, D] projection: the three gradients land in one tensor of its layout."""
 
     @staticmethod
-    def forward(ctx, qkv, key_lengths, causal, scale):
+    def forward(ctx, qkv, key_lengths, causal, scale, plan):
         q, k, v = qkv.unbind(2)
-        out, lse, lo = K.attention_fwd(q, k, v, causal, scale, key_lengths, keep=True)
+        out, lse, lo = K.attention_fwd(plan, q, k, v, causal, scale, key_lengths, keep=True)
         ctx.save_for_backward(qkv, out, lo, lse, key_lengths)
-        ctx.causal, ctx.scale = causal, scale
+        ctx.causal, ctx.scale, ctx.plan = causal, scale, plan
         return out
 
     @staticmethod
@@ -920,8 +921,8 @@ class _AttentionQKV(Function):
     def backward(ctx, dout):
         qkv, out, lo, lse, lengths = ctx.saved_tensors
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        K.attention_bwd(*qkv.unbind(2), out, lo, K._chunked(dout.to(qkv.dtype)), lse, ctx.causal, ctx.scale, lengths, *dqkv.unbind(2))
-        return dqkv, None, None, None
+        K.attention_bwd(ctx.plan, *qkv.unbind(2), out, lo, K.chunked_heads(dout), lse, ctx.causal, ctx.scale, lengths, *dqkv.unbind(2))
+        return dqkv, None, None, None, None
 
 
 def _lengths32(key_lengths: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -942,45 +943,46 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     keys is Lq = 1.  A query that sees no key gives zeros.  Inside the keys a query may be compared with, values must be finite: masked
     ones enter the products with a weight of zero.  D: a multiple of 8 (bfloat16) or 4 (float32), at most 128.  Differentiable once in
     q, k and v; ``scale`` is 1 / sqrt(D) where it is not given."""
-    K._dev(q, k, v, key_lengths)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise CoinHipError("attention: q, k and v are [B, L, H, D]")
+    K._dev(q, k, v)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     lengths = _lengths32(key_lengths)
-    q, k, v = K._chunked(q), K._chunked(k), K._chunked(v)
+    q, k, v = K.chunked_heads(q), K.chunked_heads(k), K.chunked_heads(v)
+    plan = K.attention_plan(q, k, v)
     if _wants_grad(q, k, v):
-        return _Attention.apply(q, k, v, lengths, bool(causal), scale)
-    return K.attention_fwd(q, k, v, causal, scale, lengths)[0]
+        return _Attention.apply(q, k, v, lengths, bool(causal), scale, plan)
+    return K.attention_fwd(plan, q, k, v, causal, scale, lengths)[0]
 
 
 def attention_qkv(qkv: torch.Tensor, heads: int, *, causal: bool = False, scale: Optional[float] = None,
                   key_lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
     """`attention` of one sequence's tokens among themselves on the projection qkv [B, L, 3 * heads * D] ([3][heads][D] along the last axis)
     -> [B, L, heads * D]; one gradient of qkv's layout."""
-    K._dev(qkv, key_lengths)
+    K._dev(qkv)
     if qkv.dim() != 3 or heads <= 0 or qkv.shape[2] % (3 * heads):
         raise CoinHipError(f"attention_qkv: [B, L, 3 * {heads} * D] expected, got {tuple(qkv.shape)}")
     b, l, w = qkv.shape
     x = qkv.reshape(b, l, 3, heads, w // (3 * heads))
     scale = x.shape[-1] ** -0.5 if scale is None else float(scale)
-    if x.stride(4) != 1 or x.data_ptr() & 15 or any(n > 1 and (s * x.element_size()) & 15 for n, s in zip(x.shape[:4], x.stride()[:4])):
-        x = x.contiguous()
-        x = x.clone() if x.data_ptr() & 15 else x
+    x = K.chunked_heads(x)
     lengths = _lengths32(key_lengths)
+    q, k, v = x.unbind(2)
+    plan = K.attention_plan(q, k, v, packed=True)
     if _wants_grad(x):
-        out = _AttentionQKV.apply(x, lengths, bool(causal), scale)
+        out = _AttentionQKV.apply(x, lengths, bool(causal), scale, plan)
     else:
-        out = K.attention_fwd(*x.unbind(2), causal, scale, lengths)[0]
+        out = K.attention_fwd(plan, q, k, v, causal, scale, lengths)[0]
     return out.reshape(b, l, w // 3)
 
 
 class _ResidualNorm(Function):
+    # the operands keep their own shapes here: views outside would be autograd nodes of their own, four more per call
     @staticmethod
     def forward(ctx, x, y, gate, pw, pb, nw, nb, cfg):
-        rows_per_gate, has_post, post_eps, has_pre, pre_eps, rms, scale, branch_dtype = cfg
-        post = (pw, pb, post_eps) if has_post else None
-        pre = (nw, nb, pre_eps) if has_pre else None
-        r, h, stats = K.residual_norm_fwd(x, y, gate, rows_per_gate, post, pre, rms, scale, branch_dtype, True)
+        rows_per_gate, post_eps, pre_eps, rms, scale, branch_dtype = cfg
+        r, h, stats = K.residual_norm_fwd(x, y, gate, rows_per_gate, (pw, pb, post_eps) if post_eps is not None else None,
+                                          (nw, nb, pre_eps) if pre_eps is not None else None, rms, scale, branch_dtype, True)
         ctx.cfg = cfg
         ctx.save_for_backward(x, y, gate, pw, pb, nw, stats)
         ctx.set_materialize_grads(False)
@@ -989,22 +991,18 @@ class _ResidualNorm(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dr, dh):
-        x, y, gate, pw, pb, nw, stats = ctx.saved_tensors
-        rows_per_gate, has_post, post_eps, has_pre, pre_eps, rms, scale, branch_dtype = ctx.cfg
-        need = ctx.needs_input_grad
         if dr is None and dh is None:
             return (None,) * 8
-        dr = dr.to(x.dtype).contiguous() if dr is not None else None
-        dh = dh.to(branch_dtype).contiguous() if dh is not None else None
+        x, y, gate, pw, pb, nw, stats = ctx.saved_tensors
+        rows_per_gate, post_eps, pre_eps, rms, scale, branch_dtype = ctx.cfg
+        nx, ny, ngate, npw, npb, nnw, nnb, _ = ctx.needs_input_grad
         # without a gate, a norm behind the branch or a scale, the branch's gradient IS the stream's
-        same = y is not None and gate is None and not has_post and scale == 1.0 and y.dtype == x.dtype
-        want = [need[0] or (same and need[1]), need[1] and not same, need[2], need[3], need[4], need[5] and dh is not None, need[6] and dh is not None]
-        g = K.residual_norm_bwd(x, y, gate, rows_per_gate, (pw, pb, post_eps) if has_post else None, (nw, None, pre_eps) if has_pre else None, rms, scale,
-                                stats, dr, dh, branch_dtype, want)
-        dx, dy, dgate, dpw, dpb, dnw, dnb = g
-        if same:
-            dy = dx if need[1] else None
-        return (dx if need[0] else None, dy, dgate, dpw, dpb, dnw, dnb, None)
+        same = y is not None and gate is None and post_eps is None and scale == 1.0 and y.dtype == x.dtype
+        dx, dy, dgate, dpw, dpb, dnw, dnb = K.residual_norm_bwd(
+            x, y, gate, rows_per_gate, (pw, pb, post_eps) if post_eps is not None else None, (nw, None, pre_eps) if pre_eps is not None else None, rms, scale,
+            stats, dr.contiguous() if dr is not None else None, dh.contiguous() if dh is not None else None, branch_dtype,
+            (nx or (same and ny), ny and not same, ngate, npw, npb, nnw and dh is not None, nnb and dh is not None))
+        return (dx if nx else None, (dx if ny else None) if same else dy, dgate, dpw, dpb, dnw, dnb, None)
 
 
 def _norm_of(norm: Optional[torch.nn.Module], d: int, x: torch.Tensor):
@@ -1026,7 +1024,7 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_nor
     dimensions followed by ones and D (a gate for each sequence), float32 or bfloat16.  Streams are float32 or bfloat16; branches (y and h)
     float32 or bfloat16, bfloat16 on a bfloat16 stream; ``branch_dtype`` (default: y's, else the compute dtype) is h's.  h is the norm of r
     before r is rounded to the stream's type.  D at most 8192.  Differentiable once in x, y, gate and the norms' parameters."""
-    K._dev(x, y, gate)
+    K._dev(x)
     d = x.shape[-1] if x.dim() else 0
     if x.dim() < 1 or d < 1 or d > 8192:
         raise CoinHipError(f"residual_norm: rows of 1 to 8192 elements, got {tuple(x.shape)}")
@@ -1045,8 +1043,7 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_nor
         raise CoinHipError("residual_norm: a bfloat16 stream takes bfloat16 branches")
     if not abs(float(scale)) < float("inf"):
         raise CoinHipError(f"residual_norm: scale {scale}")
-    pw = pb = nw = nb = None
-    post_eps = pre_eps = 0.0
+    pw = pb = nw = nb = post_eps = pre_eps = None
     kinds = set()
     if post_norm is not None:
         pw, pb, post_eps, rms = _norm_of(post_norm, d, x)
@@ -1057,7 +1054,7 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_nor
     if len(kinds) > 1:
         raise CoinHipError("residual_norm: both norms are LayerNorms or both are RMSNorms")
     m = x.numel() // d
-    rows_per_gate, g2 = max(m, 1), None
+    rows_per_gate = max(m, 1)
     if gate is not None:
         if gate.dtype not in (torch.float32, torch.bfloat16):
             raise CoinHipError(f"residual_norm: gate is {gate.dtype} (float32 / bfloat16 only)")
@@ -1070,51 +1067,59 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_nor
             cut -= 1
         if lead[:cut] != list(x.shape[:cut]):
             raise CoinHipError(f"residual_norm: gate {tuple(gate.shape)} is not x's leading dimensions followed by ones and {d} (x {tuple(x.shape)})")
-        g2 = gate.contiguous().view(-1, d)
-        rows_per_gate = max(m // max(g2.shape[0], 1), 1)
+        rows_per_gate = max(m // max(gate.numel() // d, 1), 1)
     if m == 0:   # no rows: nothing to launch, every gradient of a sum over them is zero
         zero = sum((t.sum() * 0.0 for t in (gate, pw, pb, nw, nb) if t is not None and t.requires_grad), 0.0)
         r = x if y is None else x + (y * scale).to(x.dtype) + (zero.to(x.dtype) if torch.is_tensor(zero) else zero)
         return r, None if pre_norm is None else r.to(branch_dtype) * 1.0 + (zero.to(branch_dtype) if torch.is_tensor(zero) else zero)
-    x2, y2 = x.reshape(m, d).contiguous(), y.reshape(m, d).contiguous() if y is not None else None
-    cfg = (rows_per_gate, post_norm is not None, post_eps, pre_norm is not None, pre_eps, True in kinds, float(scale), branch_dtype)
-    if _wants_grad(x2, y2, g2, pw, pb, nw, nb):
-        r, h = _ResidualNorm.apply(x2, y2, g2, pw, pb, nw, nb, cfg)
+    x, y, gate = (t if t is None or t.is_contiguous() else t.contiguous() for t in (x, y, gate))
+    rms = True in kinds
+    if _wants_grad(x, y, gate, pw, pb, nw, nb):
+        r, h = _ResidualNorm.apply(x, y, gate, pw, pb, nw, nb, (rows_per_gate, post_eps, pre_eps, rms, float(scale), branch_dtype))
     else:
         post, pre = (pw, pb, post_eps) if post_norm is not None else None, (nw, nb, pre_eps) if pre_norm is not None else None
-        r, h, _ = K.residual_norm_fwd(x2, y2, g2, rows_per_gate, post, pre, cfg[5], cfg[6], branch_dtype, False)
-    return x if y is None else r.view(x.shape), None if h is None else h.view(x.shape)
+        r, h, _ = K.residual_norm_fwd(x, y, gate, rows_per_gate, post, pre, rms, float(scale), branch_dtype, False)
+    return x if y is None else r, h
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` [..., K] as [M, K] rows of one pitch, the last dimension contiguous."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    s0, s1 = t.stride()
+    return t if s1 == 1 and (s0 >= t.shape[1] or t.shape[0] == 1) else t.contiguous()
 
 
 class _FusedLinear(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, wq, act):
         n, k = wq.shape
-        xr, wr = K.chunked_rows(x), K.chunked_rows(wq)
         need = ctx.needs_input_grad
-        y_dtype = residual.dtype if residual is not None else x.dtype
-        y, slope = K.linear_fwd(xr, wr, k, bias, act, residual, y_dtype, act != ACT_NONE and (need[0] or need[1] or need[2]))
+        xr, wr = K.chunked_rows(_rows(x)), K.chunked_rows(wq)
+        y, slope = K.linear_fwd(xr, wr, k, bias, act, _rows(residual) if residual is not None else None, residual.dtype if residual is not None else x.dtype,
+                                act != ACT_NONE and (need[0] or need[1] or need[2]))
         ctx.save_for_backward(xr if need[1] else None, wr if need[0] else None, slope)
-        ctx.n, ctx.k, ctx.dtype, ctx.dw_dtype, ctx.db_dtype = n, k, x.dtype, weight.dtype, bias.dtype if bias is not None else None
-        return y
+        ctx.n, ctx.k, ctx.shape, ctx.dtype, ctx.dw_dtype, ctx.db_dtype = n, k, x.shape, x.dtype, weight.dtype, bias.dtype if bias is not None else None
+        return y.view(x.shape[:-1] + (n,)) if x.dim() != 2 else y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         xr, wr, slope = ctx.saved_tensors
-        need = ctx.needs_input_grad
+        need_x, need_w, need_b, need_res, _, _ = ctx.needs_input_grad
         dx = dw = db = None
-        if need[0] or need[1] or need[2]:
-            products = need[0] or need[1]
-            if dy.stride(1) != 1 or (dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]):
-                dy = dy.contiguous()
-            as_is = products and slope is None and dy.dtype == ctx.dtype and K.chunked_ok(dy)   # dz is dy
-            dz = None
-            if not as_is or need[2]:
-                dz, db = K.linear_dz(dy, slope, ctx.dtype, products and not as_is, ctx.db_dtype if need[2] else None)
+        if need_x or need_w or need_b:
+            products = need_x or need_w
+            g = _rows(dy)
+            as_is = products and slope is None and g.dtype == ctx.dtype and K.chunked_ok(g)   # dz is dy
+            dz = g
+            if not as_is or need_b:
+                dz, db = K.linear_dz(g, slope, ctx.dtype, products and not as_is, ctx.db_dtype if need_b else None)
             if products:
-                dx, dw = K.linear_bwd(dy if as_is else dz, xr, wr, ctx.n, ctx.k, need[0], ctx.dw_dtype if need[1] else None)
-        return dx, dw, db, (dy if need[3] else None), None, None
+                dx, dw = K.linear_bwd(g if as_is else dz, xr, wr, ctx.n, ctx.k, need_x, ctx.dw_dtype if need_w else None)
+                if need_x and len(ctx.shape) != 2:
+                    dx = dx.view(ctx.shape)
+        return dx, dw, db, (dy if need_res else None), None, None
 
 
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, act: int = ACT_NONE,
@@ -1125,7 +1130,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     (the autocast dtype, else x's: bfloat16 or float32) with float32 sums; a float32 master weight is read through its bfloat16 shadow and
     receives a float32 gradient.  ``residual`` [..., N] of the compute dtype, or float32, decides the output's dtype.  Any sizes and strides
     (rows that are not whole 16-byte chunks are copied first).  Differentiable once in x, weight, bias and residual."""
-    K._dev(x, weight, bias, residual)
+    K._dev(x, weight)
     if act not in (ACT_NONE, ACT_RELU, ACT_GELU, ACT_QUICK_GELU, ACT_SILU):
         raise CoinHipError(f"fused_linear: activation {act}")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1 or (bias is not None and bias.shape != (weight.shape[0],)):
@@ -1152,13 +1157,9 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         zero = sum((t.sum() * 0.0 for t in (weight, bias) if t is not None and t.requires_grad), 0.0)
         out = x.new_zeros(shape) + x.sum() * 0.0 + (zero.to(dt) if torch.is_tensor(zero) else zero)
         return out if residual is None else residual + out.to(residual.dtype)
-    x2 = x.reshape(m, k)
-    r2 = None
-    if residual is not None:
-        r2 = residual.reshape(m, n)
-        if r2.stride(1) != 1 or (m > 1 and r2.stride(0) < n):
-            r2 = r2.contiguous()
-    bias = bias.contiguous() if bias is not None else None
-    if _wants_grad(x2, weight, bias, r2):
-        return _FusedLinear.apply(x2, weight, bias, r2, wq.detach(), act).view(shape)
-    return K.linear_fwd(K.chunked_rows(x2), K.chunked_rows(wq), k, bias, act, r2, r2.dtype if r2 is not None else dt, False)[0].view(shape)
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if _wants_grad(x, weight, bias, residual):
+        return _FusedLinear.apply(x, weight, bias, residual, wq.detach(), act)
+    r2 = _rows(residual) if residual is not None else None
+    return K.linear_fwd(K.chunked_rows(_rows(x)), K.chunked_rows(wq), k, bias, act, r2, dt if r2 is None else r2.dtype, False)[0].view(shape)

@@ -511,7 +511,7 @@ int coin_residual_norm_bwd(const void* x, const void* y, const void* gate, int64
  * layers, float32 for float32 ones.
  * x and W rows: 16-byte aligned, leading dimensions of whole 16-byte chunks that hold the row's last chunk whole (COIN_EALIGN; coin_pad_rows
  * makes such rows); where K is not a multiple of a chunk (8 bf16, 4 f32) the rest of the last chunk holds ZEROS.  The same for dz below.
- * 130 rows' span below 2^31 bytes (COIN_ESHAPE).  workspace: coin_linear_workspace_bytes, 16-byte aligned. */
+ * 260 rows' span below 2^31 bytes (COIN_ESHAPE).  workspace: coin_linear_workspace_bytes, 16-byte aligned. */
 size_t coin_linear_workspace_bytes(int64_t M, int N, int K, int dtype, int backward);
 int coin_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int act, const void* residual,
                     int64_t ldr, void* y, int64_t ldy, int y_dtype, void* slope, int64_t ld_slope, int64_t M, int N, int K, int dtype,
