@@ -21,8 +21,7 @@
 // registers, so P and dS are B operands again).  That is 7 products where one launch would take 5, but every sum has one owner: no atomics,
 // the same bits every time, and the heads that share a key head are summed in registers.
 //
-// K, V, Q, dO tiles go to LDS by the range-checked LDS-DMA, two buffers, one barrier per tile.  16-byte chunk c of row r sits at chunk
-// c ^ g(r): eight rows' chunk c (a row fragment) and four rows' 32-byte segment (a transposed fragment) both fall on different banks.
+// K, V, Q, dO tiles go to LDS by the range-checked LDS-DMA into swizzled images (mfma_tile.h), two buffers, one barrier per tile.
 // float32 tensors take the same kernels with 32x32x2 float32 matrix instructions: four of them use one 16-byte fragment.
 #include "common.h"
 #include "mfma_tile.h"
@@ -40,7 +39,8 @@ struct AttnArgs {
   const int* lengths;                 // [B] or null
   int64_t qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];   // element strides: sequence, token, head
   int B, Lq, Lk, Hkv, g, D, R;
-  int causal, splits, chunk;          // splits of the keys (forward) or of the rows (dK, dV), `chunk` of them each
+  int causal, splits, chunk;          // splits of the keys (forward; `chunk` keys each) or of the rows (dK, dV)
+  int pair;                           // dK, dV, causal: workgroups of the first of two rounds (0: no order of its own)
   float scale, c;                     // c = scale * log2 e
   float *part, *part_ml;
 };
@@ -51,7 +51,7 @@ template <typename T, int ROWB, int ND>
 __device__ __forceinline__ void mma_t(f32x16 (&acc)[ND], const char* img, int row0, const f32x16& p, int lane) {
   const int half = lane >> 5;
   if constexpr (sizeof(T) == 2) {
-    const int q4 = (lane >> 2) & 3, p4 = lane & 3, lrow = half * 4 + q4, sw = swz<ROWB>(lrow);
+    const int q4 = (lane >> 2) & 3, p4 = lane & 3, lrow = half * 4 + q4, sw0 = swz<ROWB>(lrow), sw1 = swz<ROWB>(lrow + 8);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       bf16x8 pf;
@@ -60,9 +60,10 @@ __device__ __forceinline__ void mma_t(f32x16 (&acc)[ND], const char* img, int ro
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) {
         const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + (p4 >> 1);
-        const char* a0 = img + (row0 + 16 * s + lrow) * ROWB + ((chunk ^ sw) << 4) + (p4 & 1) * 8;
+        const char* a0 = img + (row0 + 16 * s + lrow) * ROWB + ((chunk ^ sw0) << 4) + (p4 & 1) * 8;
+        const char* a1 = img + (row0 + 16 * s + lrow + 8) * ROWB + ((chunk ^ sw1) << 4) + (p4 & 1) * 8;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a0);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a0 + 8 * ROWB));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a1);
         const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), pf, acc[dt], 0, 0, 0);
       }
@@ -118,7 +119,7 @@ struct Cfg {
 
 // ------------------------------------------------------------------------------------------------------------------------------ forward
 template <typename T, int DP, int NW, bool SPLIT>
-__global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs p) {
+__global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_fwd_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
   constexpr int ROWB = C::ROWB, KT = C::KT;
   __shared__ __attribute__((aligned(1024))) char lds[4 * C::TILE];
@@ -299,7 +300,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
 
 // ----------------------------------------------------------------------------------------------------------------------- backward: dQ, D
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs p) {
+__global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_dq_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
   constexpr int ROWB = C::ROWB, KT = C::KT;
   __shared__ __attribute__((aligned(1024))) char lds[4 * C::TILE];
@@ -401,7 +402,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs p)
 
 // -------------------------------------------------------------------------------------------------------------------- backward: dK and dV
 template <typename T, int DP, int NW, bool SPLIT>
-__global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs p) {
+__global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_dkv_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
   constexpr int ROWB = C::ROWB, KT = C::KT;
   __shared__ __attribute__((aligned(1024))) char lds[4 * C::TILE];
@@ -409,12 +410,17 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs p
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nbh = p.B * p.Hkv;
+  // causal: the first keys have the most rows, so their workgroups come first; `pair` workgroups make one round over the chip, and the second
+  // round runs backwards: the CU that got the longest gets the shortest beside it
   int id = blockIdx.x, split = 0;
+  if (p.pair && id >= p.pair) id = p.pair + (int)gridDim.x - 1 - id;
+  const int tile = id / (nbh * (SPLIT ? p.splits : 1));
+  id -= tile * (nbh * (SPLIT ? p.splits : 1));
   if (SPLIT) {
-    split = id % p.splits;
-    id /= p.splits;
+    split = id / nbh;
+    id -= split * nbh;
   }
-  const int tile = id / nbh, bh = id % nbh;   // causal: the first keys have the most rows
+  const int bh = id;
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int n = keys_of(p, b), nchunk = p.D / C::EL;
   const int k0 = tile * NW * 32, kw = k0 + wave * 32, key = kw + (lane & 31);
@@ -426,10 +432,10 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs p
     t0 = i0 > 0 ? i0 * p.g : 0;
   }
   int te = k0 < n ? p.R : 0;
-  if (SPLIT) {
-    const int s0 = split * p.chunk;
-    if (te > s0 + p.chunk) te = s0 + p.chunk;
-    if (t0 < s0) t0 = s0;
+  if (SPLIT && t0 < te) {   // this split's share of the tile's rows
+    const int share = ((te - t0 + p.splits - 1) / p.splits + 31) / 32 * 32, first = t0;
+    t0 = first + split * share < te ? first + split * share : te;
+    te = t0 + share < te ? t0 + share : te;
   }
   const int h0 = hk * p.g;
   f32x4 kf[C::NC], vf[C::NC];
@@ -495,36 +501,33 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs p
       const char* qimg = lds + buf * 2 * C::TILE;
       const char* gimg = qimg + C::TILE;
       const bool masked = kw + 32 > row_limit(p, tt, n);   // rows behind `te` have L = inf: their P is 0 without a mask
-#pragma unroll
+#pragma unroll 1
       for (int s = 0; s < C::NS; ++s) {
-        f32x16 st = zero16(), dp = zero16();
+        f32x16 st = zero16();
 #pragma unroll
-        for (int cc = 0; cc < C::NC; ++cc) {
-          mma<T>(st, frag<ROWB>(qimg, s * 32 + (lane & 31), 2 * cc + half), kf[cc]);
-          mma<T>(dp, frag<ROWB>(gimg, s * 32 + (lane & 31), 2 * cc + half), vf[cc]);
-        }
+        for (int cc = 0; cc < C::NC; ++cc) mma<T>(st, frag<ROWB>(qimg, s * 32 + (lane & 31), 2 * cc + half), kf[cc]);
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
           const int at = s * 32 + 8 * r4 + 4 * half;
           const f32x4 L = *reinterpret_cast<const f32x4*>(&stat[buf][0][at]);
-          const f32x4 De = *reinterpret_cast<const f32x4*>(&stat[buf][1][at]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = r4 * 4 + e;
-            st[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], c, -L[e]));
-            dp[r] = st[r] * (dp[r] - De[e]);
-          }
-          if (masked) {
+          for (int e = 0; e < 4; ++e) st[r4 * 4 + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r4 * 4 + e], c, -L[e]));
+          if (masked) {   // a masked P is 0, and so is its dS
             const f32x4 lm = *reinterpret_cast<const f32x4*>(&stat[buf][2][at]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const bool see = key < __float_as_int(lm[e]);
-              st[r4 * 4 + e] = see ? st[r4 * 4 + e] : 0.f;
-              dp[r4 * 4 + e] = see ? dp[r4 * 4 + e] : 0.f;
-            }
+            for (int e = 0; e < 4; ++e) st[r4 * 4 + e] = key < __float_as_int(lm[e]) ? st[r4 * 4 + e] : 0.f;
           }
         }
         mma_t<T, ROWB, C::ND>(dv, gimg, s * 32, st, lane);
+        f32x16 dp = zero16();
+#pragma unroll
+        for (int cc = 0; cc < C::NC; ++cc) mma<T>(dp, frag<ROWB>(gimg, s * 32 + (lane & 31), 2 * cc + half), vf[cc]);
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 De = *reinterpret_cast<const f32x4*>(&stat[buf][1][s * 32 + 8 * r4 + 4 * half]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dp[r4 * 4 + e] = st[r4 * 4 + e] * (dp[r4 * 4 + e] - De[e]);
+        }
         mma_t<T, ROWB, C::ND>(dk, qimg, s * 32, dp, lane);
       }
     }
@@ -594,22 +597,18 @@ static int fwd_splits(int64_t wgs, int Lk, int* chunk) {
 
 static int fwd_waves(int64_t R, int64_t nbh) { return (R + 127) / 128 * nbh >= cus() ? 4 : 1; }
 
-static int dkv_splits(int64_t wgs, int64_t R, int* chunk) {
-  *chunk = (int)R;
-  if (wgs >= cus() || R <= 512) return 1;
-  int64_t s = (2 * cus() + wgs - 1) / wgs, most = (R + 255) / 256;
-  if (s > most) s = most;
-  if (s <= 1) return 1;
-  int c = (int)((R + s - 1) / s);
-  c = (c + 63) / 64 * 64;
-  *chunk = c;
-  return (int)((R + c - 1) / c);
+// Row splits of the dK, dV launch: its workgroups (128 keys of a head, 250 registers a thread) run two to a CU, and a causal head's are
+// unequal.  Two rounds' worth at least while there are 512 rows for each; measured on 2 x 4001 causal tokens, 16 heads over 4, D 128:
+static int dkv_splits(int64_t wgs, int64_t R) {
+  int64_t s = (2 * cus() + wgs - 1) / wgs;
+  if (s > R / 512) s = R / 512;
+  return s < 1 ? 1 : (int)s;
 }
 
 static int dkv_waves(int64_t Lk, int64_t nbh) { return (Lk + 127) / 128 * nbh >= cus() ? 4 : 1; }
 
 struct Plan {
-  int fw, fsplits, fchunk, kw, ksplits, kchunk;
+  int fw, fsplits, fchunk, kw, ksplits;
   size_t fwd_bytes, bwd_bytes;
 };
 
@@ -621,7 +620,7 @@ static Plan make_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv
   if (p.fsplits == 1) p.fchunk = (int)Lk;
   p.fwd_bytes = p.fsplits > 1 ? (size_t)p.fsplits * nbh * R * (D + 2) * sizeof(float) : 0;
   p.kw = dkv_waves(Lk, nbh);
-  p.ksplits = dkv_splits((Lk + p.kw * 32 - 1) / (p.kw * 32) * nbh, R, &p.kchunk);
+  p.ksplits = dkv_splits((Lk + p.kw * 32 - 1) / (p.kw * 32) * nbh, R);
   p.bwd_bytes = (size_t)nbh * R * sizeof(float);
   p.bwd_bytes = (p.bwd_bytes + 255) / 256 * 256;
   if (p.ksplits > 1) p.bwd_bytes += (size_t)p.ksplits * nbh * Lk * 2 * D * sizeof(float);
@@ -663,7 +662,7 @@ static void launch_fwd(const AttnArgs& a, const Plan& pl, hipStream_t st) {
 }
 
 template <typename T, int DP>
-static void launch_bwd(const AttnArgs& a, const Plan& pl, hipStream_t st) {
+static void launch_bwd(AttnArgs a, const Plan& pl, hipStream_t st) {
   const int64_t nbh = (int64_t)a.B * a.Hkv;
   if (a.R > 0) {
     const unsigned grid = (unsigned)((a.R + pl.fw * 32 - 1) / (pl.fw * 32) * nbh);
@@ -672,6 +671,7 @@ static void launch_bwd(const AttnArgs& a, const Plan& pl, hipStream_t st) {
   }
   if (a.Lk > 0) {
     const unsigned grid = (unsigned)((a.Lk + pl.kw * 32 - 1) / (pl.kw * 32) * nbh * pl.ksplits);
+    a.pair = a.causal && (int)grid > cus() && (int)grid <= 2 * cus() ? cus() : 0;
     if (pl.ksplits > 1) {
       if (pl.kw == 1) attention_dkv_kernel<T, DP, 1, true><<<grid, 64, 0, st>>>(a);
       else attention_dkv_kernel<T, DP, 4, true><<<grid, 256, 0, st>>>(a);
@@ -760,7 +760,7 @@ extern "C" int coin_attention_bwd(const void* q, const int64_t* q_strides, const
   a.lo = (bf16_t*)const_cast<void*>(out_lo);
   a.q = q; a.k = k; a.v = v; a.o = out; a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.lse = const_cast<float*>(lse); a.lengths = key_lengths;
   a.B = B; a.Lq = Lq; a.Lk = Lk; a.Hkv = Hkv; a.g = g; a.D = D; a.R = Lq * g;
-  a.causal = causal != 0; a.splits = pl.ksplits; a.chunk = pl.kchunk; a.scale = scale; a.c = scale * LOG2E;
+  a.causal = causal != 0; a.splits = pl.ksplits; a.scale = scale; a.c = scale * LOG2E;
   a.delta = (float*)workspace;
   a.part = (float*)((char*)workspace + ((size_t)B * Hkv * a.R * sizeof(float) + 255) / 256 * 256);
   if (dtype == COIN_BF16) launch<bf16_t>(a, pl, true, (hipStream_t)stream);

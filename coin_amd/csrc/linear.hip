@@ -161,8 +161,7 @@ __device__ __forceinline__ void load_bias(const LinArgs& p, float (&b)[8], int c
   for (int i = 0; i < 8; ++i) b[i] = p.bias && col + i < p.N ? (p.bias_f32 ? ((const float*)p.bias)[col + i] : (float)((const bf16_t*)p.bias)[col + i]) : 0.f;
 }
 
-constexpr int BKB = 64;   // bytes of the contraction in a stage
-constexpr int NST = 3;    // stages of the ring
+constexpr int BKB = 128;   // bytes of the contraction in a stage: whole cache lines (64-byte rows cost a quarter of the rate)
 
 // One operand of a stage: E rows (or columns) of the output, BKB bytes of the contraction.  ACROSS: the contraction runs across the rows
 template <typename T, bool ACROSS, int E, int NW>
@@ -205,41 +204,72 @@ struct Operand {
   }
 };
 
-// all but the youngest stage's PER DMA instructions of this wave have landed, or all of them
-template <int PER>
-__device__ __forceinline__ void wait_stage(bool another) {
-  static_assert(PER == 2 || PER == 4 || PER == 6, "");
-  if (!another) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  else if (PER == 2) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)" ::: "memory");
-  else if (PER == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
+// XCD-aware order: workgroups b, b + 8, ... share an XCD and take neighbouring items of a contiguous eighth of the list; the list walks groups
+// of 8 tile rows column by column, so what runs together shares 8 row panels and a few column panels in the XCD's L2
+__device__ __forceinline__ void tile_of(const LinArgs& p, int& tm, int& tn, int& piece) {
+  const int nwg = gridDim.x, q = nwg >> 3, r = nwg & 7, x = blockIdx.x & 7, i = blockIdx.x >> 3;
+  const int item = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + i;
+  piece = item % p.split;
+  const int tile = item / p.split, per = 8 * p.tiles_n, grp = tile / per, in = tile - grp * per;
+  const int gm = p.tiles_m - grp * 8 < 8 ? p.tiles_m - grp * 8 : 8;
+  tm = grp * 8 + in % gm;
+  tn = in / gm;
 }
 
-// C tile TM x TN by four waves (2 x 2), each TM / 2 x TN / 2 in 32 x 32 accumulators; a ring of three stages, two in flight under the third.
-// 256 x 128: 72 KiB of LDS and 128 accumulator registers, two workgroups per CU: one's epilogue, prologue and barriers run under the
-// other's matrix instructions.
-template <typename T, bool AA, bool BA, int TM, int TN>
+// rows mp .. mp + ROWS - 1 of the output from the epilogue image (ROWS x TN float32, 16-byte chunk c of row r at c ^ (r & 7)); NT threads
+template <typename T, int ROWS, int TN, int NT>
+__device__ __forceinline__ void finish_rows(const LinArgs& p, const char* lds, int mp, int n0, int piece) {
+  constexpr int TPR = TN / 8, RPP = NT / TPR;
+  const int c8 = threadIdx.x % TPR, col = n0 + c8 * 8;
+  if (col >= p.N) return;
+  float bias[8];
+  if (p.split == 1) load_bias(p, bias, col);
+  for (int rr = threadIdx.x / TPR; rr < ROWS && mp + rr < p.M; rr += RPP) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(lds + rr * (TN * 4) + (((2 * c8) ^ (rr & 7)) << 4));
+    const f32x4 y = *reinterpret_cast<const f32x4*>(lds + rr * (TN * 4) + (((2 * c8 + 1) ^ (rr & 7)) << 4));
+    if (p.split > 1) {
+      float* o = p.part + ((int64_t)piece * p.M + mp + rr) * p.N + col;
+      if (p.N % 8 == 0) {
+        *reinterpret_cast<f32x4*>(o) = x;
+        *reinterpret_cast<f32x4*>(o + 4) = y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (col + i < p.N) o[i] = i < 4 ? x[i & 3] : y[i & 3];
+      }
+    } else {
+      float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      finish8<T>(p, v, bias, mp + rr, col);
+    }
+  }
+}
+
+// one 32 x 32 accumulator into the image: lane & 31 = row, registers = columns
+template <int TN>
+__device__ __forceinline__ void put_tile(char* lds, const f32x16& acc, int row0, int col0, int lane) {
+  const int row = row0 + (lane & 31), half = lane >> 5;
+#pragma unroll
+  for (int r = 0; r < 16; r += 4) {
+    const int ch = (col0 + 2 * r + 4 * half) >> 2;
+    *reinterpret_cast<f32x4*>(lds + row * (TN * 4) + ((ch ^ (row & 7)) << 4)) = (f32x4){acc[r], acc[r + 1], acc[r + 2], acc[r + 3]};
+  }
+}
+
+// C tile TS x TS by four waves (2 x 2), each (TS / 2)^2 in 32 x 32 accumulators, a ring of NST stages.  128 x 128 x 2 stages: 64 KiB of LDS,
+// two workgroups per CU, one's epilogue and barriers under the other's matrix instructions; 64 x 64 x 3: 48 KiB, three per CU
+template <typename T, bool AA, bool BA, int TS, int NST>
 __global__ __launch_bounds__(256, 2) void linear_gemm_kernel(const LinArgs p) {
-  using OA = Operand<T, AA, TM, 4>;
-  using OB = Operand<T, BA, TN, 4>;
-  constexpr int BK = OA::BK, STAGE = OA::BYTES + OB::BYTES, WM = TM / 64, WN = TN / 64, PER = STAGE / 4096;
-  constexpr int RING = NST * STAGE, PASS = TM * TN * 4 <= RING ? 1 : 2, IMG = TM * TN * 4 / PASS;   // passes and bytes of the epilogue image
-  __shared__ __attribute__((aligned(1024))) char lds[RING > IMG ? RING : IMG];
-  const int lane = threadIdx.x & 63, half = lane >> 5;
+  using OA = Operand<T, AA, TS, 4>;
+  using OB = Operand<T, BA, TS, 4>;
+  constexpr int BK = OA::BK, STAGE = OA::BYTES + OB::BYTES, W = TS / 64;
+  __shared__ __attribute__((aligned(1024))) char lds[NST * STAGE];
+  static_assert(NST * STAGE >= TS * TS * 4 && (NST == 2 || (NST == 3 && STAGE == 4 * 4096)), "");
+  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave >> 1, wc = wave & 1;
-  // XCD-aware order: workgroups b, b + 8, ... share an XCD and take neighbouring items of a contiguous eighth of the list; the list walks
-  // groups of 8 tile rows column by column, so what runs together shares 8 row panels and a few column panels in the XCD's L2
-  int item;
-  {
-    const int nwg = gridDim.x, q = nwg >> 3, r = nwg & 7, x = blockIdx.x & 7, i = blockIdx.x >> 3;
-    item = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + i;
-  }
-  const int piece = item % p.split, tile = item / p.split;
-  const int per = 8 * p.tiles_n, grp = tile / per, in = tile - grp * per;
-  const int gm = p.tiles_m - grp * 8 < 8 ? p.tiles_m - grp * 8 : 8;
-  const int tm = grp * 8 + in % gm, tn = in / gm;
-  const int m0 = tm * TM, n0 = tn * TN;
+  int tm, tn, piece;
+  tile_of(p, tm, tn, piece);
+  const int m0 = tm * TS, n0 = tn * TS;
   const int nk = (p.K + BK - 1) / BK;
   const int kb = (int)((int64_t)piece * nk / p.split), ke = (int)((int64_t)(piece + 1) * nk / p.split);
   auto stage = [&](int kt, int slot) {
@@ -247,76 +277,147 @@ __global__ __launch_bounds__(256, 2) void linear_gemm_kernel(const LinArgs p) {
     OA::stage(d, (const T*)p.A, p.lda, m0, p.M, kt * BK, p.K, wave, lane);
     OB::stage(d + OA::BYTES, (const T*)p.B, p.ldb, n0, p.N, kt * BK, p.K, wave, lane);
   };
-  f32x16 acc[WM][WN];
+  f32x16 acc[W][W];
 #pragma unroll
-  for (int i = 0; i < WM; ++i)
+  for (int i = 0; i < W; ++i)
 #pragma unroll
-    for (int j = 0; j < WN; ++j) acc[i][j] = zero16();
-  if (kb < ke) stage(kb, 0);
-  if (kb + 1 < ke) stage(kb + 1, 1);
+    for (int j = 0; j < W; ++j) acc[i][j] = zero16();
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s)
+    if (kb + s < ke) stage(kb + s, s);
   int slot = 0;
   for (int kt = kb; kt < ke; ++kt) {
-    wait_stage<PER>(kt + 1 < ke);   // stage kt has landed
-    P8_BAR();                       // for every wave, and nobody reads the slot of stage kt - 1 any more
-    if (kt + 2 < ke) stage(kt + 2, slot == 0 ? 2 : slot - 1);
+    // stage kt has landed: a wave's four DMA instructions of one younger stage may be under way
+    if (NST == 3 && kt + 1 < ke) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    P8_BAR();   // for every wave, and nobody reads the slot of stage kt - 1 any more
+    if (kt + NST - 1 < ke) stage(kt + NST - 1, slot == 0 ? NST - 1 : slot - 1);
     const char* la = lds + slot * STAGE;
     const char* lb = la + OA::BYTES;
 #pragma unroll
     for (int s = 0; s < BKB / 32; ++s) {
-      f32x4 a[WM], b[WN];
+      f32x4 a[W], b[W];
 #pragma unroll
-      for (int j = 0; j < WN; ++j) b[j] = OB::frag_at(lb, wc * (TN / 2) + j * 32, s, lane);
+      for (int j = 0; j < W; ++j) b[j] = OB::frag_at(lb, wc * (TS / 2) + j * 32, s, lane);
 #pragma unroll
-      for (int i = 0; i < WM; ++i) a[i] = OA::frag_at(la, wr * (TM / 2) + i * 32, s, lane);
+      for (int i = 0; i < W; ++i) a[i] = OA::frag_at(la, wr * (TS / 2) + i * 32, s, lane);
 #pragma unroll
-      for (int i = 0; i < WM; ++i)
+      for (int i = 0; i < W; ++i)
 #pragma unroll
-        for (int j = 0; j < WN; ++j) mma<T>(acc[i][j], b[j], a[i]);   // swapped: lane = output row, registers = 4 consecutive columns
+        for (int j = 0; j < W; ++j) mma<T>(acc[i][j], b[j], a[i]);   // swapped: lane = output row, registers = 4 consecutive columns
     }
-    slot = slot == 2 ? 0 : slot + 1;
+    slot = slot == NST - 1 ? 0 : slot + 1;
   }
-  // the ring becomes the epilogue image, TM / PASS rows of TN float32, 16-byte chunk c of row r at c ^ (r & 7)
-  constexpr int ROWS = TM / PASS, TPR = TN / 8, RPP = 256 / TPR;
-  const int c8 = threadIdx.x % TPR, col = n0 + c8 * 8;
-  float bias[8];
-  if (p.split == 1) load_bias(p, bias, col);
+  P8_LDS_SYNC();   // every wave is done with the ring: it becomes the epilogue image
 #pragma unroll
-  for (int pass = 0; pass < PASS; ++pass) {
-    P8_LDS_SYNC();   // every wave is done with what the image overwrites
-    if (PASS == 1 || wr == pass) {
+  for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int i = 0; i < WM; ++i) {
-        const int row = (PASS == 1 ? wr * (TM / 2) : 0) + i * 32 + (lane & 31);
+    for (int j = 0; j < W; ++j) put_tile<TS>(lds, acc[i][j], wr * (TS / 2) + i * 32, wc * (TS / 2) + j * 32, lane);
+  P8_LDS_SYNC();
+  finish_rows<T, TS, TS, 256>(p, lds, m0, n0, piece);
+}
+
+// C tile 256 x 256 by eight waves in two groups of four (one wave of each per SIMD), one workgroup per CU, two K-tiles of 64 in LDS, each of
+// four half-tiles (A or B, low or high 128 rows, 16 KiB).  A wave owns a 64 x 32 piece of every (A half, B half) quadrant and walks them in
+// four phases {read fragments, issue one half-tile's DMA; barrier; eight matrix instructions; barrier}:
+//   1: reads B low, A low     2: reads B high     3: reads A high     4: reads nothing;   products  Al Bl, Al Bh, Ah Bh, Ah Bl
+// Group 1 runs one barrier behind group 0: one group's matrix instructions run while the other reads.  In barrier intervals, group 0's phase
+// i of K-tile g reads at 8 g + 2 (i - 1), group 1 one later; so A low and B low are free from 8 g + 2 on, B high from 8 g + 4, A high from
+// 8 g + 6, and their K-tile g + 2 is issued in phases 3, 2, 4 of K-tile g and 1 of K-tile g + 1.  The order of issue is Bl Al Bh Ah, and each is
+// read by everybody in the phase after the wait that leaves the five youngest half-tiles (ten instructions of a wave) under way: fourteen
+// intervals to land.  K-tiles behind the last are issued too, out of range: they write zeros that nobody reads and keep the count.
+// (bfloat16 alone: float32 matrix instructions are sixteen times slower, and 128 x 128 tiles already feed them)
+template <bool AA, bool BA>
+__global__ __launch_bounds__(512, 2) void linear_gemm256_kernel(const LinArgs p) {
+  using T = bf16_t;
+  using OA = Operand<T, AA, 128, 8>;
+  using OB = Operand<T, BA, 128, 8>;
+  constexpr int BK = OA::BK, HALF = OA::BYTES, STAGE = 4 * HALF;   // Al | Ah | Bl | Bh
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  static_assert(HALF == 16384 && OB::BYTES == HALF, "two DMA instructions of a wave a half-tile");
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = wave >> 2, wr = group, wc = wave & 3;
+  int tm, tn, piece;
+  tile_of(p, tm, tn, piece);
+  const int m0 = tm * 256, n0 = tn * 256;
+  const int nk = (p.K + BK - 1) / BK;
+  auto stage_a = [&](int kt, int hi) {
+    OA::stage(lds + (kt & 1) * STAGE + hi * HALF, (const T*)p.A, p.lda, m0 + hi * 128, p.M, kt * BK, p.K, wave, lane);
+  };
+  auto stage_b = [&](int kt, int hi) {
+    OB::stage(lds + (kt & 1) * STAGE + (2 + hi) * HALF, (const T*)p.B, p.ldb, n0 + hi * 128, p.N, kt * BK, p.K, wave, lane);
+  };
+  f32x16 acc[2][2][2];
 #pragma unroll
-        for (int j = 0; j < WN; ++j)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; r += 4) {
-            const int ch = (wc * (TN / 2) + j * 32 + 2 * r + 4 * half) >> 2;
-            *reinterpret_cast<f32x4*>(lds + row * (TN * 4) + ((ch ^ (row & 7)) << 4)) = (f32x4){acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
-          }
-      }
-    }
+    for (int j = 0; j < 2; ++j) acc[i][j][0] = acc[i][j][1] = zero16();
+  f32x4 a[2][4], b[2][4];
+  // `landed`: for group 0 behind the products, for group 1 behind the reads -- in either case ahead of the barrier that ends an odd interval
+  auto multiply = [&](int ah, int bh) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (group) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+    P8_BAR();
+    P8_SCHED();
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mma<T>(acc[ah][bh][i], b[bh][s], a[i][s]);
+    __builtin_amdgcn_s_setprio(0);
+    P8_SCHED();
+    if (!group) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+    P8_BAR();
+    P8_SCHED();
+  };
+  auto read_a = [&](const char* img) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) a[i][s] = OA::frag_at(img, wr * 64 + i * 32, s, lane);
+  };
+  auto read_b = [&](const char* img, int bh) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) b[bh][s] = OB::frag_at(img, wc * 32, s, lane);
+  };
+  stage_b(0, 0);
+  stage_a(0, 0);
+  stage_b(0, 1);
+  stage_a(0, 1);
+  stage_b(1, 0);
+  stage_a(1, 0);
+  stage_b(1, 1);
+  asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+  P8_BAR();
+  if (group) P8_BAR();
+  for (int kt = 0; kt < nk; ++kt) {
+    const char* img = lds + (kt & 1) * STAGE;
+    read_b(img + 2 * HALF, 0);
+    read_a(img);
+    stage_a(kt + 1, 1);
+    multiply(0, 0);
+    read_b(img + 3 * HALF, 1);
+    stage_b(kt + 2, 0);
+    multiply(0, 1);
+    read_a(img + HALF);
+    stage_a(kt + 2, 0);
+    multiply(1, 1);
+    stage_b(kt + 2, 1);
+    multiply(1, 0);
+  }
+  if (!group) P8_BAR();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // epilogue image: 128 rows (the low, then the high half of A) of 256 float32 columns
+#pragma unroll
+  for (int ah = 0; ah < 2; ++ah) {
     P8_LDS_SYNC();
-    if (col >= p.N) continue;
-    const int mp = m0 + pass * ROWS;
-    for (int rr = threadIdx.x / TPR; rr < ROWS && mp + rr < p.M; rr += RPP) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(lds + rr * (TN * 4) + (((2 * c8) ^ (rr & 7)) << 4));
-      const f32x4 y = *reinterpret_cast<const f32x4*>(lds + rr * (TN * 4) + (((2 * c8 + 1) ^ (rr & 7)) << 4));
-      if (p.split > 1) {
-        float* o = p.part + ((int64_t)piece * p.M + mp + rr) * p.N + col;
-        if (p.N % 8 == 0) {
-          *reinterpret_cast<f32x4*>(o) = x;
-          *reinterpret_cast<f32x4*>(o + 4) = y;
-        } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (col + i < p.N) o[i] = i < 4 ? x[i & 3] : y[i & 3];
-        }
-      } else {
-        float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-        finish8<T>(p, v, bias, mp + rr, col);
-      }
-    }
+    for (int bh = 0; bh < 2; ++bh)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) put_tile<256>(lds, acc[ah][bh][i], wr * 64 + i * 32, bh * 128 + wc * 32, lane);
+    P8_LDS_SYNC();
+    finish_rows<T, 128, 256, 512>(p, lds, m0 + ah * 128, n0, piece);
   }
 }
 
@@ -465,22 +566,23 @@ constexpr int64_t SPAN = 0x7fffffff;
 constexpr int CUS = 256;   // MI355X
 
 struct Tiling {
-  int tm, tn, split;
+  int ts, split;
 };
 
-// Tile size and K pieces of one product: the largest of 256 x 128, 128 x 128 and 64 x 64 tiles that still fills the chip (two workgroups
-// per CU of the first, one of the second); if even 64 x 64 tiles are fewer than the CUs, the contraction is cut so that they become two per
-// CU, in pieces of at least eight stages
+// Tile size and K pieces of one product.  bfloat16: 256 x 256 tiles where their last round over the CUs is at least three quarters full on average;
+// else 128 x 128 where they fill the CUs, else 64 x 64; if even those are fewer than the CUs, the contraction is cut so that they become two
+// per CU, in pieces of at least four stages
 static Tiling plan(int64_t M, int64_t N, int64_t K, int es) {
-  const int64_t tn = (N + 127) / 128, nk = (K * es + BKB - 1) / BKB;
-  if ((M + 255) / 256 * tn >= 2 * CUS) return {256, 128, 1};
-  const bool big = (M + 127) / 128 * tn >= CUS;
-  const int64_t t = big ? (M + 127) / 128 * tn : ((M + 63) / 64) * ((N + 63) / 64);
+  const int64_t nk = (K * es + BKB - 1) / BKB;
+  const int64_t t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 127) / 128 * ((N + 127) / 128);
+  const int64_t rounds = (t256 + CUS - 1) / CUS;
+  if (es == 2 && 4 * t256 >= 3 * rounds * CUS) return {256, 1};
+  const int ts = t128 >= CUS ? 128 : 64;
+  const int64_t t = ts == 128 ? t128 : (M + 63) / 64 * ((N + 63) / 64);
   int64_t s = t >= CUS ? 1 : 2 * CUS / t;
-  if (s > nk / 8) s = nk / 8;
+  if (s > nk / 4) s = nk / 4;
   if (s > 64) s = 64;
-  if (s < 1) s = 1;
-  return {big ? 128 : 64, big ? 128 : 64, (int)s};
+  return {ts, s < 1 ? 1 : (int)s};
 }
 
 static size_t part_bytes(int64_t M, int64_t N, int64_t K, int es) {
@@ -492,12 +594,15 @@ template <typename T, bool AA, bool BA>
 static void run_gemm(LinArgs a, hipStream_t st) {
   const Tiling t = plan(a.M, a.N, a.K, sizeof(T));
   a.split = t.split;
-  a.tiles_m = (a.M + t.tm - 1) / t.tm;
-  a.tiles_n = (a.N + t.tn - 1) / t.tn;
+  a.tiles_m = (a.M + t.ts - 1) / t.ts;
+  a.tiles_n = (a.N + t.ts - 1) / t.ts;
   const unsigned grid = (unsigned)(a.tiles_m * a.tiles_n * a.split);
-  if (t.tm == 256) linear_gemm_kernel<T, AA, BA, 256, 128><<<grid, 256, 0, st>>>(a);
-  else if (t.tm == 128) linear_gemm_kernel<T, AA, BA, 128, 128><<<grid, 256, 0, st>>>(a);
-  else linear_gemm_kernel<T, AA, BA, 64, 64><<<grid, 256, 0, st>>>(a);
+  if constexpr (sizeof(T) == 2) {
+    if (t.ts == 256) linear_gemm256_kernel<AA, BA><<<grid, 512, 0, st>>>(a);
+  }
+  if (t.ts == 256) return;
+  if (t.ts == 128) linear_gemm_kernel<T, AA, BA, 128, 2><<<grid, 256, 0, st>>>(a);
+  else linear_gemm_kernel<T, AA, BA, 64, 3><<<grid, 256, 0, st>>>(a);
   if (a.split > 1) linear_join_kernel<T><<<(unsigned)(((int64_t)a.M * ((a.N + 7) / 8) + 255) / 256), 256, 0, st>>>(a);
 }
 

@@ -21,11 +21,14 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
-// 16-byte chunk c of row r of an image with ROWB-byte rows sits at chunk c ^ swz(r): eight rows' chunk c (a row fragment) and four rows'
-// 32-byte segment (a transposed fragment) both fall on different banks
+// 16-byte chunk c of row r of an image with ROWB-byte rows sits at chunk c ^ swz(r).  LDS serves 256 bytes (64 banks) at a time: the chunk c
+// of 16 consecutive rows (a row fragment's quarter) and 64 bytes of 4 consecutive rows (half of a transposed fragment) must fall on
+// different banks.  Rows of 256 bytes and more all start on bank 0: four bits of the row, the lowest two on the 64-byte segment; shorter rows
+// lie on different banks by themselves as far as they go.  (Swizzles of eight 16-byte slots, as 128 bytes at a time would ask for, left every
+// second LDS cycle a conflict.)
 template <int ROWB>
 __device__ __forceinline__ int swz(int r) {
-  return ROWB == 64 ? ((r >> 1) & 1) << 1 | ((r >> 2) & 1) : ((r & 3) << 1) | ((r >> 2) & 1);
+  return ROWB == 64 ? (r >> 2) & 3 : ROWB == 128 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3) : (r & 3) << 2 | ((r >> 2) & 3);
 }
 
 // acc[i][j] += sum over the 16-byte fragments: A row i = lane & 31, B column j = lane & 31, contraction = 8 bf16 / 4 floats per lane half
