@@ -40,18 +40,17 @@ struct AttnArgs {
   int64_t qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];   // element strides: sequence, token, head
   int B, Lq, Lk, Hkv, g, D, R;
   int causal, splits, chunk;          // splits of the keys (forward; `chunk` keys each) or of the rows (dK, dV)
-  int pair;                           // dK, dV, causal: workgroups of the first of two rounds (0: no order of its own)
   float scale, c;                     // c = scale * log2 e
   float *part, *part_ml;
 };
 
 // acc[dt]^T[d][col] += sum over the 32 image rows row0 .. row0 + 31 of image[row][d] * p[row][col], p in accumulator registers:
 // register r of lane half h holds row 8 (r >> 2) + 4 h + (r & 3)
-template <typename T, int ROWB, int ND>
+template <typename T, typename I, int ND>
 __device__ __forceinline__ void mma_t(f32x16 (&acc)[ND], const char* img, int row0, const f32x16& p, int lane) {
   const int half = lane >> 5;
   if constexpr (sizeof(T) == 2) {
-    const int q4 = (lane >> 2) & 3, p4 = lane & 3, lrow = half * 4 + q4, sw0 = swz<ROWB>(lrow), sw1 = swz<ROWB>(lrow + 8);
+    const int q4 = (lane >> 2) & 3, p4 = lane & 3, lrow = half * 4 + q4;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       bf16x8 pf;
@@ -60,8 +59,8 @@ __device__ __forceinline__ void mma_t(f32x16 (&acc)[ND], const char* img, int ro
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) {
         const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + (p4 >> 1);
-        const char* a0 = img + (row0 + 16 * s + lrow) * ROWB + ((chunk ^ sw0) << 4) + (p4 & 1) * 8;
-        const char* a1 = img + (row0 + 16 * s + lrow + 8) * ROWB + ((chunk ^ sw1) << 4) + (p4 & 1) * 8;
+        const char* a0 = img + I::row_at(row0 + 16 * s) + I::row_at(lrow) + ((chunk ^ I::key(lrow)) << 4) + (p4 & 1) * 8;
+        const char* a1 = img + I::row_at(row0 + 16 * s + 8) + I::row_at(lrow) + ((chunk ^ I::key(lrow + 8)) << 4) + (p4 & 1) * 8;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a0);
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a1);
         const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -71,11 +70,11 @@ __device__ __forceinline__ void mma_t(f32x16 (&acc)[ND], const char* img, int ro
   } else {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int lrow = 8 * (r >> 2) + 4 * half + (r & 3), sw = swz<ROWB>(lrow);
+      const int lrow = 8 * (r >> 2) + 4 * half + (r & 3);
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) {
         const int chunk = dt * 8 + ((lane & 31) >> 2);
-        const float a = *reinterpret_cast<const float*>(img + (row0 + lrow) * ROWB + ((chunk ^ sw) << 4) + (lane & 3) * 4);
+        const float a = *reinterpret_cast<const float*>(img + I::row_at(row0) + I::row_at(lrow) + ((chunk ^ I::key(lrow)) << 4) + (lane & 3) * 4);
         acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[dt], 0, 0, 0);
       }
     }
@@ -114,13 +113,15 @@ struct Cfg {
   static constexpr int KT = ROWB <= 256 ? 64 : 32;  // rows of a staged tile: two double-buffered tiles stay within 64 KiB
   static constexpr int NS = KT / 32, ND = DP / 32;
   static constexpr int EL = 16 / (int)sizeof(T);    // elements of a chunk
-  static constexpr int TILE = KT * ROWB;
+  using I = Img<ROWB, KT, ROWB == 256>;             // row0 of a fragment is a multiple of 8: row_at adds up
+  static constexpr int TILE = I::BYTES;
 };
 
 // ------------------------------------------------------------------------------------------------------------------------------ forward
 template <typename T, int DP, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_fwd_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
+  using I = typename C::I;
   constexpr int ROWB = C::ROWB, KT = C::KT;
   __shared__ __attribute__((aligned(1024))) char lds[4 * C::TILE];
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -154,8 +155,8 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
   const unsigned kst = (unsigned)(p.ks[1] * sizeof(T)), vst = (unsigned)(p.vs[1] * sizeof(T));
   auto stage = [&](int kt, int buf) {
     char* d = lds + buf * 2 * C::TILE;
-    stage_tile<ROWB, KT, NW>(d, kbase + (int64_t)kt * p.ks[1], n - kt, nchunk, wave, lane, [&](int r) { return (unsigned)r * kst; });
-    stage_tile<ROWB, KT, NW>(d + C::TILE, vbase + (int64_t)kt * p.vs[1], n - kt, nchunk, wave, lane, [&](int r) { return (unsigned)r * vst; });
+    stage_tile<ROWB, KT, NW, ROWB == 256>(d, kbase + (int64_t)kt * p.ks[1], n - kt, nchunk, wave, lane, [&](int r) { return (unsigned)r * kst; });
+    stage_tile<ROWB, KT, NW, ROWB == 256>(d + C::TILE, vbase + (int64_t)kt * p.vs[1], n - kt, nchunk, wave, lane, [&](int r) { return (unsigned)r * vst; });
   };
   f32x16 o[C::ND];
 #pragma unroll
@@ -174,8 +175,9 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
 #pragma unroll
     for (int s = 0; s < C::NS; ++s) {
       st[s] = zero16();
+      if (sizeof(T) == 2 || kt + s * 32 < wmax)   // float32 products are dear: 32 keys that no row of the wave sees cost their mask alone
 #pragma unroll
-      for (int cc = 0; cc < C::NC; ++cc) mma<T>(st[s], frag<ROWB>(kimg, s * 32 + (lane & 31), 2 * cc + half), qf[cc]);
+        for (int cc = 0; cc < C::NC; ++cc) mma<T>(st[s], I::frag(kimg, s * 32 + (lane & 31), 2 * cc + half), qf[cc]);
     }
     if (kt + KT > wmin) {
 #pragma unroll
@@ -208,7 +210,8 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
       }
     l += ls;
 #pragma unroll
-    for (int s = 0; s < C::NS; ++s) mma_t<T, ROWB, C::ND>(o, vimg, s * 32, st[s], lane);
+    for (int s = 0; s < C::NS; ++s)
+      if (sizeof(T) == 2 || kt + s * 32 < wmax) mma_t<T, I, C::ND>(o, vimg, s * 32, st[s], lane);
   }
   l += __shfl_xor(l, 32, 64);
   if (!live) return;
@@ -252,7 +255,8 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
     }
 }
 
-// one wave per row: the splits' sums joined with their maxima
+// one wave per row: the splits' sums joined with their maxima, in split order.  Lane s first holds split s's maximum and sum, so that the loads
+// of the partial rows do not wait for one another
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
   const int lane = threadIdx.x & 63;
@@ -261,23 +265,32 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
   float m = -INFINITY;
   bool bad = false;
   for (int s = lane; s < p.splits; s += 64) {
-    const float l = p.part_ml[(s * rows + row) * 2 + 1], mm = p.part_ml[(s * rows + row) * 2];
-    if (l != 0.f) m = fmaxf(m, mm);
-    bad |= !(l == l);
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + row) * 2);
+    if (ml.y != 0.f) m = fmaxf(m, ml.x);
+    bad |= !(ml.y == ml.y);
   }
   m = wave_reduce_max(m);
   bad = __any(bad);
   float a0 = 0.f, a1 = 0.f, l = 0.f;
   const int d = lane * 2;   // head dimensions are even and <= 128
-  for (int s = 0; s < p.splits; ++s) {
-    const float ls = p.part_ml[(s * rows + row) * 2 + 1];
-    if (!(ls > 0.f)) continue;
-    const float w = __builtin_amdgcn_exp2f(p.part_ml[(s * rows + row) * 2] - m);
-    l += ls * w;
-    if (d < p.D) {
-      const float2 v = *reinterpret_cast<const float2*>(p.part + (s * rows + row) * p.D + d);
-      a0 = __builtin_fmaf(v.x, w, a0);
-      a1 = __builtin_fmaf(v.y, w, a1);
+  for (int s0 = 0; s0 < p.splits; s0 += 64) {
+    float w = 0.f, ls = 0.f;
+    if (s0 + lane < p.splits) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((s0 + lane) * rows + row) * 2);
+      if (ml.y > 0.f) {
+        w = __builtin_amdgcn_exp2f(ml.x - m);
+        ls = ml.y * w;
+      }
+    }
+    l += wave_reduce_sum(ls);
+    const int ns = p.splits - s0 < 64 ? p.splits - s0 : 64;
+#pragma unroll 8
+    for (int s = 0; s < ns; ++s) {
+      const float ws = __shfl(w, s, 64);
+      float2 v = make_float2(0.f, 0.f);
+      if (ws != 0.f && d < p.D) v = *reinterpret_cast<const float2*>(p.part + ((s0 + s) * rows + row) * p.D + d);   // sums of a split without keys are not there
+      a0 = __builtin_fmaf(v.x, ws, a0);
+      a1 = __builtin_fmaf(v.y, ws, a1);
     }
   }
   if (bad) l = __builtin_nanf("");
@@ -302,6 +315,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_dq_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
+  using I = typename C::I;
   constexpr int ROWB = C::ROWB, KT = C::KT;
   __shared__ __attribute__((aligned(1024))) char lds[4 * C::TILE];
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -327,8 +341,8 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
   const unsigned kst = (unsigned)(p.ks[1] * sizeof(T)), vst = (unsigned)(p.vs[1] * sizeof(T));
   auto stage = [&](int kt, int buf) {
     char* d = lds + buf * 2 * C::TILE;
-    stage_tile<ROWB, KT, NW>(d, kbase + (int64_t)kt * p.ks[1], n - kt, nchunk, wave, lane, [&](int r) { return (unsigned)r * kst; });
-    stage_tile<ROWB, KT, NW>(d + C::TILE, vbase + (int64_t)kt * p.vs[1], n - kt, nchunk, wave, lane, [&](int r) { return (unsigned)r * vst; });
+    stage_tile<ROWB, KT, NW, ROWB == 256>(d, kbase + (int64_t)kt * p.ks[1], n - kt, nchunk, wave, lane, [&](int r) { return (unsigned)r * kst; });
+    stage_tile<ROWB, KT, NW, ROWB == 256>(d + C::TILE, vbase + (int64_t)kt * p.vs[1], n - kt, nchunk, wave, lane, [&](int r) { return (unsigned)r * vst; });
   };
   if (ke > 0) stage(0, 0);
   f32x4 qf[C::NC], gf[C::NC];
@@ -370,11 +384,12 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
     const bool masked = kt + KT > wmin;
 #pragma unroll
     for (int s = 0; s < C::NS; ++s) {
+      if (sizeof(T) == 4 && kt + s * 32 >= wmax) break;
       f32x16 st = zero16(), dp = zero16();
 #pragma unroll
       for (int cc = 0; cc < C::NC; ++cc) {
-        mma<T>(st, frag<ROWB>(kimg, s * 32 + (lane & 31), 2 * cc + half), qf[cc]);
-        mma<T>(dp, frag<ROWB>(vimg, s * 32 + (lane & 31), 2 * cc + half), gf[cc]);
+        mma<T>(st, I::frag(kimg, s * 32 + (lane & 31), 2 * cc + half), qf[cc]);
+        mma<T>(dp, I::frag(vimg, s * 32 + (lane & 31), 2 * cc + half), gf[cc]);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -385,7 +400,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[r] = kt + s * 32 + 8 * (r >> 2) + 4 * half + (r & 3) < lim ? st[r] : 0.f;
       }
-      mma_t<T, ROWB, C::ND>(dq, kimg, s * 32, st, lane);
+      mma_t<T, I, C::ND>(dq, kimg, s * 32, st, lane);
     }
   }
   if (!live) return;
@@ -404,16 +419,20 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
 template <typename T, int DP, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_dkv_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
-  constexpr int ROWB = C::ROWB, KT = C::KT;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * C::TILE];
+  // bfloat16, D 128: the fragments of K (32 registers), of V (32) and the two accumulators (128) leave too little of 256 registers (spilled:
+  // 690 us, 590 us with V in LDS); V's 32 KiB beside tiles of 32 rows still let two workgroups on a CU
+  constexpr bool VL = sizeof(T) == 2 && DP == 128 && NW == 4;
+  constexpr int ROWB = C::ROWB, KT = VL ? 32 : C::KT, NS = KT / 32;
+  using I = Img<ROWB, KT, ROWB == 256>;
+  using IV = Img<ROWB, NW * 32, ROWB == 256>;
+  constexpr int TILE = I::BYTES;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + (VL ? IV::BYTES : 0)];
+  char* const vimg = lds + 4 * TILE;
   __shared__ __attribute__((aligned(16))) float stat[2][3][KT];   // L, D and the limit of each staged row
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nbh = p.B * p.Hkv;
-  // causal: the first keys have the most rows, so their workgroups come first; `pair` workgroups make one round over the chip, and the second
-  // round runs backwards: the CU that got the longest gets the shortest beside it
-  int id = blockIdx.x, split = 0;
-  if (p.pair && id >= p.pair) id = p.pair + (int)gridDim.x - 1 - id;
+  int id = blockIdx.x, split = 0;   // causal: the first keys have the most rows, so their workgroups come first
   const int tile = id / (nbh * (SPLIT ? p.splits : 1));
   id -= tile * (nbh * (SPLIT ? p.splits : 1));
   if (SPLIT) {
@@ -438,22 +457,28 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
     te = t0 + share < te ? t0 + share : te;
   }
   const int h0 = hk * p.g;
-  f32x4 kf[C::NC], vf[C::NC];
+  f32x4 kf[C::NC], vf[VL ? 1 : C::NC];
   load_frags<C::NC>(kf, (const char*)((const T*)p.k + b * p.ks[0] + (int64_t)key * p.ks[1] + hk * p.ks[2]), live, nchunk, half);
-  load_frags<C::NC>(vf, (const char*)((const T*)p.v + b * p.vs[0] + (int64_t)key * p.vs[1] + hk * p.vs[2]), live, nchunk, half);
+  if constexpr (VL) {
+    const unsigned vst = (unsigned)(p.vs[1] * sizeof(T));
+    stage_tile<ROWB, NW * 32, NW, ROWB == 256>(vimg, (const T*)p.v + b * p.vs[0] + (int64_t)k0 * p.vs[1] + hk * p.vs[2], n - k0, nchunk, wave, lane,
+                                               [&](int r) { return (unsigned)r * vst; });
+  } else {
+    load_frags<C::NC>(vf, (const char*)((const T*)p.v + b * p.vs[0] + (int64_t)key * p.vs[1] + hk * p.vs[2]), live, nchunk, half);
+  }
   const T* qbase = (const T*)p.q + b * p.qs[0] + h0 * p.qs[2];
   const T* gbase = (const T*)p.dout + b * p.dos[0] + h0 * p.dos[2];
   const unsigned ql = (unsigned)(p.qs[1] * sizeof(T)), qh = (unsigned)(p.qs[2] * sizeof(T));
   const unsigned gl = (unsigned)(p.dos[1] * sizeof(T)), gh = (unsigned)(p.dos[2] * sizeof(T));
   auto stage = [&](int tt, int buf) {
-    char* d = lds + buf * 2 * C::TILE;
+    char* d = lds + buf * 2 * TILE;
     const int i0 = p.g == 1 ? tt : tt / p.g;
-    stage_tile<ROWB, KT, NW>(d, qbase + (int64_t)i0 * p.qs[1], te - tt, nchunk, wave, lane, [&](int r) {
+    stage_tile<ROWB, KT, NW, ROWB == 256>(d, qbase + (int64_t)i0 * p.qs[1], te - tt, nchunk, wave, lane, [&](int r) {
       if (p.g == 1) return (unsigned)r * ql;
       const int x = tt + r, i = x / p.g;
       return (unsigned)(i - i0) * ql + (unsigned)(x - i * p.g) * qh;
     });
-    stage_tile<ROWB, KT, NW>(d + C::TILE, gbase + (int64_t)i0 * p.dos[1], te - tt, nchunk, wave, lane, [&](int r) {
+    stage_tile<ROWB, KT, NW, ROWB == 256>(d + TILE, gbase + (int64_t)i0 * p.dos[1], te - tt, nchunk, wave, lane, [&](int r) {
       if (p.g == 1) return (unsigned)r * gl;
       const int x = tt + r, i = x / p.g;
       return (unsigned)(i - i0) * gl + (unsigned)(x - i * p.g) * gh;
@@ -498,14 +523,16 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
     }
     const int last = tt + KT - 1 < te ? tt + KT - 1 : te - 1;
     if (kw < row_limit(p, last, n)) {
-      const char* qimg = lds + buf * 2 * C::TILE;
-      const char* gimg = qimg + C::TILE;
+      const char* qimg = lds + buf * 2 * TILE;
+      const char* gimg = qimg + TILE;
       const bool masked = kw + 32 > row_limit(p, tt, n);   // rows behind `te` have L = inf: their P is 0 without a mask
 #pragma unroll 1
-      for (int s = 0; s < C::NS; ++s) {
+      for (int s = 0; s < NS; ++s) {
+        const int end = tt + s * 32 + 31 < last ? tt + s * 32 + 31 : last;
+        if (NS > 1 && (tt + s * 32 > last || kw >= row_limit(p, end, n))) continue;   // no row of these 32 sees a key of the wave
         f32x16 st = zero16();
 #pragma unroll
-        for (int cc = 0; cc < C::NC; ++cc) mma<T>(st, frag<ROWB>(qimg, s * 32 + (lane & 31), 2 * cc + half), kf[cc]);
+        for (int cc = 0; cc < C::NC; ++cc) mma<T>(st, I::frag(qimg, s * 32 + (lane & 31), 2 * cc + half), kf[cc]);
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
           const int at = s * 32 + 8 * r4 + 4 * half;
@@ -518,17 +545,17 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
             for (int e = 0; e < 4; ++e) st[r4 * 4 + e] = key < __float_as_int(lm[e]) ? st[r4 * 4 + e] : 0.f;
           }
         }
-        mma_t<T, ROWB, C::ND>(dv, gimg, s * 32, st, lane);
+        mma_t<T, I, C::ND>(dv, gimg, s * 32, st, lane);
         f32x16 dp = zero16();
 #pragma unroll
-        for (int cc = 0; cc < C::NC; ++cc) mma<T>(dp, frag<ROWB>(gimg, s * 32 + (lane & 31), 2 * cc + half), vf[cc]);
+        for (int cc = 0; cc < C::NC; ++cc) mma<T>(dp, I::frag(gimg, s * 32 + (lane & 31), 2 * cc + half), VL ? IV::frag(vimg, wave * 32 + (lane & 31), 2 * cc + half) : vf[VL ? 0 : cc]);
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
           const f32x4 De = *reinterpret_cast<const f32x4*>(&stat[buf][1][s * 32 + 8 * r4 + 4 * half]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) dp[r4 * 4 + e] = st[r4 * 4 + e] * (dp[r4 * 4 + e] - De[e]);
         }
-        mma_t<T, ROWB, C::ND>(dk, qimg, s * 32, dp, lane);
+        mma_t<T, I, C::ND>(dk, qimg, s * 32, dp, lane);
       }
     }
     if (more) put_stat(tt + KT, buf ^ 1, ls, de);
@@ -597,10 +624,11 @@ static int fwd_splits(int64_t wgs, int Lk, int* chunk) {
 
 static int fwd_waves(int64_t R, int64_t nbh) { return (R + 127) / 128 * nbh >= cus() ? 4 : 1; }
 
-// Row splits of the dK, dV launch: its workgroups (128 keys of a head, 250 registers a thread) run two to a CU, and a causal head's are
-// unequal.  Two rounds' worth at least while there are 512 rows for each; measured on 2 x 4001 causal tokens, 16 heads over 4, D 128:
+// Row splits of the dK, dV launch: its workgroups (128 keys of a head) run two to a CU, and a causal head's are unequal, so two rounds' worth
+// are wanted while there are 512 rows for each.  Measured on 2 x 4001 causal tokens, 16 heads over 4, D 128 (256 workgroups unsplit): no split
+// 978 us, two splits 592 + 15 us of joining, four 406 + 25, eight 425 + 45
 static int dkv_splits(int64_t wgs, int64_t R) {
-  int64_t s = (2 * cus() + wgs - 1) / wgs;
+  int64_t s = (4 * cus() + wgs - 1) / wgs;
   if (s > R / 512) s = R / 512;
   return s < 1 ? 1 : (int)s;
 }
@@ -662,7 +690,7 @@ static void launch_fwd(const AttnArgs& a, const Plan& pl, hipStream_t st) {
 }
 
 template <typename T, int DP>
-static void launch_bwd(AttnArgs a, const Plan& pl, hipStream_t st) {
+static void launch_bwd(const AttnArgs& a, const Plan& pl, hipStream_t st) {
   const int64_t nbh = (int64_t)a.B * a.Hkv;
   if (a.R > 0) {
     const unsigned grid = (unsigned)((a.R + pl.fw * 32 - 1) / (pl.fw * 32) * nbh);
@@ -671,7 +699,6 @@ static void launch_bwd(AttnArgs a, const Plan& pl, hipStream_t st) {
   }
   if (a.Lk > 0) {
     const unsigned grid = (unsigned)((a.Lk + pl.kw * 32 - 1) / (pl.kw * 32) * nbh * pl.ksplits);
-    a.pair = a.causal && (int)grid > cus() && (int)grid <= 2 * cus() ? cus() : 0;
     if (pl.ksplits > 1) {
       if (pl.kw == 1) attention_dkv_kernel<T, DP, 1, true><<<grid, 64, 0, st>>>(a);
       else attention_dkv_kernel<T, DP, 4, true><<<grid, 256, 0, st>>>(a);

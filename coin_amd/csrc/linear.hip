@@ -61,62 +61,81 @@ __device__ __forceinline__ float sigmoid_of(float x) {
   else return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
 }
 
-// act(z), and act'(z) where it is kept
+// v <- act(v) for eight values, and act'(v) into sl where SLOPE.  The activation is chosen once for the eight: a choice per value made the
+// epilogue's code larger than the instruction cache
 template <typename T, bool SLOPE>
-__device__ __forceinline__ float act_of(float z, int act, float& slope) {
-  slope = 1.f;
-  if (act == COIN_ACT_NONE) return z;
-  if (act == COIN_ACT_RELU) {
-    slope = z > 0.f ? 1.f : 0.f;
-    return z > 0.f ? z : (z != z ? z : 0.f);
+__device__ __forceinline__ void act8(float (&v)[8], float (&sl)[8], int act) {
+  if (act == COIN_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sl[i] = 1.f;
+  } else if (act == COIN_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sl[i] = v[i] > 0.f ? 1.f : 0.f;
+      v[i] = v[i] > 0.f ? v[i] : (v[i] != v[i] ? v[i] : 0.f);
+    }
+  } else if (act == COIN_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float cdf, bell;
+      normal_cdf<T>(v[i], cdf, bell);
+      if (SLOPE) sl[i] = __builtin_fmaf(v[i] * 0.39894228040143268f, bell, cdf);
+      v[i] *= cdf;
+    }
+  } else {
+    const float a = act == COIN_ACT_QUICK_GELU ? 1.702f : 1.f;   // z sigmoid(a z)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float s = sigmoid_of<T>(a * v[i]);
+      if (SLOPE) sl[i] = s * (1.f + a * v[i] * (1.f - s));
+      v[i] *= s;
+    }
   }
-  if (act == COIN_ACT_GELU) {
-    float cdf, bell;
-    normal_cdf<T>(z, cdf, bell);
-    if (SLOPE) slope = __builtin_fmaf(z * 0.39894228040143268f, bell, cdf);
-    return z * cdf;
+}
+
+// the residual's eight columns of a row; `raw`: what finish_rows fetched ahead (bfloat16 rows of whole chunks)
+__device__ __forceinline__ void residual8(const LinArgs& p, float (&r)[8], const bf16x8& raw, int64_t row, int col) {
+  const int left = p.N - col;
+  if (p.vec && !p.c_f32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (float)raw[i];
+  } else if (p.vec) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>((const float*)p.res + row * p.ldr + col);
+    const f32x4 b = *reinterpret_cast<const f32x4*>((const float*)p.res + row * p.ldr + col + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r[i] = a[i];
+      r[4 + i] = b[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      r[i] = 0.f;
+      if (i < left) r[i] = p.c_f32 ? ((const float*)p.res)[row * p.ldr + col + i] : (float)((const bf16_t*)p.res)[row * p.ldr + col + i];
+    }
   }
-  const float a = act == COIN_ACT_QUICK_GELU ? 1.702f : 1.f;   // z sigmoid(a z)
-  const float s = sigmoid_of<T>(a * z);
-  if (SLOPE) slope = s * (1.f + a * z * (1.f - s));
-  return z * s;
+}
+
+__device__ __forceinline__ bf16x8 residual_ahead(const LinArgs& p, int64_t row, int col) {
+  bf16x8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (bf16_t)0.f;
+  if (p.res && p.vec && !p.c_f32) r = *reinterpret_cast<const bf16x8*>((const bf16_t*)p.res + row * p.ldr + col);
+  return r;
 }
 
 // eight columns of one row through the epilogue: v holds the product
 template <typename T>
-__device__ __forceinline__ void finish8(const LinArgs& p, float (&v)[8], const float (&bias)[8], int64_t row, int col) {
+__device__ __forceinline__ void finish8(const LinArgs& p, float (&v)[8], const float (&bias)[8], const bf16x8& ahead, int64_t row, int col) {
   const int left = p.N - col;
   float sl[8], r[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) r[i] = 0.f;
-  if (p.res) {
-    if (p.vec) {
-      if (p.c_f32) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>((const float*)p.res + row * p.ldr + col);
-        const f32x4 b = *reinterpret_cast<const f32x4*>((const float*)p.res + row * p.ldr + col + 4);
+  if (p.res) residual8(p, r, ahead, row, col);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          r[i] = a[i];
-          r[4 + i] = b[i];
-        }
-      } else {
-        const bf16x8 a = *reinterpret_cast<const bf16x8*>((const bf16_t*)p.res + row * p.ldr + col);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = (float)a[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < left) r[i] = p.c_f32 ? ((const float*)p.res)[row * p.ldr + col + i] : (float)((const bf16_t*)p.res)[row * p.ldr + col + i];
-    }
-  }
-  if (p.slope) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_of<T, true>(v[i] + bias[i], p.act, sl[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_of<T, false>(v[i] + bias[i], p.act, sl[i]);
-  }
+  for (int i = 0; i < 8; ++i) v[i] += bias[i];
+  if (p.slope) act8<T, true>(v, sl, p.act);
+  else act8<T, false>(v, sl, p.act);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] += r[i];
   if (p.vec) {
@@ -180,7 +199,7 @@ struct Operand {
   static __device__ __forceinline__ f32x4 frag_at(const char* img, int row0, int s, int lane) {
     const int half = lane >> 5;
     if constexpr (!ACROSS) {
-      return frag<BKB>(img, row0 + (lane & 31), 2 * s + half);
+      return Img<BKB, ROWS>::frag(img, row0 + (lane & 31), 2 * s + half);
     } else if constexpr (sizeof(T) == 2) {
       const int q4 = (lane >> 2) & 3, p4 = lane & 3;
       const int chunk = (row0 >> 3) + ((lane >> 4) & 1) * 2 + (p4 >> 1);
@@ -224,7 +243,14 @@ __device__ __forceinline__ void finish_rows(const LinArgs& p, const char* lds, i
   if (col >= p.N) return;
   float bias[8];
   if (p.split == 1) load_bias(p, bias, col);
-  for (int rr = threadIdx.x / TPR; rr < ROWS && mp + rr < p.M; rr += RPP) {
+  // a rolled loop: the epilogue runs once a tile, and unrolled it is larger than the instruction cache (14 us a tile of 256 x 256).  The next
+  // row's residual is on its way while this one is finished
+  const int r0 = threadIdx.x / TPR;
+  bf16x8 ahead = residual_ahead(p, mp + r0 < p.M ? mp + r0 : p.M - 1, col);
+#pragma unroll 1
+  for (int rr = r0; rr < ROWS && mp + rr < p.M; rr += RPP) {
+    const int nx = mp + rr + RPP;
+    const bf16x8 next = residual_ahead(p, nx < p.M ? nx : p.M - 1, col);
     const f32x4 x = *reinterpret_cast<const f32x4*>(lds + rr * (TN * 4) + (((2 * c8) ^ (rr & 7)) << 4));
     const f32x4 y = *reinterpret_cast<const f32x4*>(lds + rr * (TN * 4) + (((2 * c8 + 1) ^ (rr & 7)) << 4));
     if (p.split > 1) {
@@ -239,8 +265,9 @@ __device__ __forceinline__ void finish_rows(const LinArgs& p, const char* lds, i
       }
     } else {
       float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      finish8<T>(p, v, bias, mp + rr, col);
+      finish8<T>(p, v, bias, ahead, mp + rr, col);
     }
+    ahead = next;
   }
 }
 
@@ -409,16 +436,17 @@ __global__ __launch_bounds__(512, 2) void linear_gemm256_kernel(const LinArgs p)
   if (!group) P8_BAR();
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   // epilogue image: 128 rows (the low, then the high half of A) of 256 float32 columns
-#pragma unroll
-  for (int ah = 0; ah < 2; ++ah) {
+  auto half_rows = [&](const f32x16 (&c)[2][2], int mp) {
     P8_LDS_SYNC();
 #pragma unroll
     for (int bh = 0; bh < 2; ++bh)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) put_tile<256>(lds, acc[ah][bh][i], wr * 64 + i * 32, bh * 128 + wc * 32, lane);
+      for (int i = 0; i < 2; ++i) put_tile<256>(lds, c[bh][i], wr * 64 + i * 32, bh * 128 + wc * 32, lane);
     P8_LDS_SYNC();
-    finish_rows<T, 128, 256, 512>(p, lds, m0 + ah * 128, n0, piece);
-  }
+    finish_rows<T, 128, 256, 512>(p, lds, mp, n0, piece);
+  };
+  half_rows(acc[0], m0);
+  half_rows(acc[1], m0 + 128);
 }
 
 // the K pieces of eight columns of a row, in order, and the epilogue
@@ -448,7 +476,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const LinArgs p) {
     }
   }
   load_bias(p, bias, col);
-  finish8<T>(p, v, bias, row, col);
+  finish8<T>(p, v, bias, residual_ahead(p, row, col), row, col);
 }
 
 // dz = dy o act' (rows of ldz elements, zeros behind N) and the column sums of dz per block of rows.  32 threads x 8 columns, 8 rows at a time

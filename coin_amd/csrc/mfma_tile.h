@@ -42,25 +42,35 @@ __device__ __forceinline__ void mma(f32x16& acc, const f32x4& a, const f32x4& b)
   }
 }
 
-// row fragment: 16 bytes of row `row`, chunk `chunk` of an image with ROWB-byte rows
-template <int ROWB>
-__device__ __forceinline__ f32x4 frag(const char* img, int row, int chunk) {
-  return *reinterpret_cast<const f32x4*>(img + row * ROWB + ((chunk ^ swz<ROWB>(row)) << 4));
-}
+// An image of `ROWS` rows.  PAD: every 1 KiB (one DMA instruction's rows) is followed by 16 bytes, which takes the place of the swizzle's lower
+// two bits for 256-byte rows: what is left of the swizzle touches a chunk's upper bits alone, so a fragment's addresses are four registers and
+// constant offsets instead of sixteen registers.
+template <int ROWB, int ROWS, bool PAD = false>
+struct Img {
+  static_assert(!PAD || ROWB == 256, "");
+  static constexpr int BLOCK = PAD ? 1040 : 1024, BYTES = ROWB * ROWS / 1024 * BLOCK;
+  static __device__ __forceinline__ int key(int row) { return PAD ? (row & 3) << 2 : swz<ROWB>(row); }
+  static __device__ __forceinline__ int row_at(int row) { return PAD ? (row >> 2) * BLOCK + (row & 3) * ROWB : row * ROWB; }
+  // row fragment: 16 bytes of row `row`, chunk `chunk`
+  static __device__ __forceinline__ f32x4 frag(const char* img, int row, int chunk) {
+    return *reinterpret_cast<const f32x4*>(img + row_at(row) + ((chunk ^ key(row)) << 4));
+  }
+};
 
 // rows 0 .. ROWS - 1 of a tile -> swizzled LDS image; rows >= nvalid and chunks >= nchunk arrive as zeros.  `off(row)` = byte offset of a
 // row behind `base` (below 2^31: checked on the host)
-template <int ROWB, int ROWS, int NW, typename OFF>
+template <int ROWB, int ROWS, int NW, bool PAD = false, typename OFF>
 __device__ __forceinline__ void stage_tile(char* dst, const void* base, int nvalid, int nchunk, int wave, int lane, const OFF& off) {
+  using I = Img<ROWB, ROWS, PAD>;
   constexpr int LPR = ROWB / 16, RPI = 64 / LPR, NI = ROWS / RPI;
   static_assert(ROWS % RPI == 0 && NI % NW == 0, "");
 #pragma unroll
   for (int i = 0; i < NI / NW; ++i) {
     const int inst = wave * (NI / NW) + i;
     const int row = inst * RPI + lane / LPR;
-    const int ch = (lane % LPR) ^ swz<ROWB>(row);
+    const int ch = (lane % LPR) ^ I::key(row);
     const unsigned o = row < nvalid && ch < nchunk ? off(row) + (unsigned)ch * 16u : P8_OOB;
-    blds16(base, 0x7fffffffu, o, 0, dst + inst * 1024);
+    blds16(base, 0x7fffffffu, o, 0, dst + inst * I::BLOCK);
   }
 }
 
