@@ -612,7 +612,7 @@ static int cus() { return 256; }   // MI355X
 // Keys per split of the forward: workgroups of one wave (32 rows) would leave the chip idle when there are few rows
 static int fwd_splits(int64_t wgs, int Lk, int* chunk) {
   *chunk = Lk;
-  if (wgs >= 2 * cus() || Lk <= 512) return 1;
+  if (wgs <= 0 || wgs >= 2 * cus() || Lk <= 512) return 1;
   int64_t s = (8 * cus() + wgs - 1) / wgs, most = (Lk + 255) / 256;
   if (s > most) s = most;
   if (s <= 1) return 1;
@@ -628,6 +628,7 @@ static int fwd_waves(int64_t R, int64_t nbh) { return (R + 127) / 128 * nbh >= c
 // are wanted while there are 512 rows for each.  Measured on 2 x 4001 causal tokens, 16 heads over 4, D 128 (256 workgroups unsplit): no split
 // 978 us, two splits 592 + 15 us of joining, four 406 + 25, eight 425 + 45
 static int dkv_splits(int64_t wgs, int64_t R) {
+  if (wgs <= 0) return 1;
   int64_t s = (4 * cus() + wgs - 1) / wgs;
   if (s > R / 512) s = R / 512;
   return s < 1 ? 1 : (int)s;

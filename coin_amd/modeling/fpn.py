@@ -104,11 +104,11 @@ def build_clip_resnet_fpn_backbone(cfg, input_shape=None):
 
 
 class SwinFPN(_FPNBackbone):
-    def __init__(self, embed_dim: int = 96, depths=(2, 2, 6, 2), num_heads=(3, 6, 12, 24), window: int = 7, out_channels: int = 256):
+    def __init__(self, embed_dim: int = 96, depths=(2, 2, 6, 2), num_heads=(3, 6, 12, 24), window: int = 7, out_channels: int = 256, fused: bool = False):
         super().__init__()
         from .swin import SwinTransformer
 
-        self.bottom_up = SwinTransformer(embed_dim=embed_dim, depths=depths, num_heads=num_heads, window_size=window)
+        self.bottom_up = SwinTransformer(embed_dim=embed_dim, depths=depths, num_heads=num_heads, window_size=window, fused=fused)
         self.fpn = FPN(["res2", "res3", "res4", "res5"], [embed_dim * 2 ** i for i in range(4)], out_channels)
 
     def bottom_up_features(self, image):
@@ -118,7 +118,8 @@ class SwinFPN(_FPNBackbone):
 @BACKBONE_REGISTRY.register()
 def build_swint_fpn_backbone(cfg, input_shape=None):
     s = cfg.MODEL.SWIN
-    return SwinFPN(embed_dim=s.EMBED_DIM, depths=tuple(s.DEPTHS), num_heads=tuple(s.NUM_HEADS), window=s.WINDOW_SIZE, out_channels=cfg.MODEL.FPN.OUT_CHANNELS)
+    return SwinFPN(embed_dim=s.EMBED_DIM, depths=tuple(s.DEPTHS), num_heads=tuple(s.NUM_HEADS), window=s.WINDOW_SIZE, out_channels=cfg.MODEL.FPN.OUT_CHANNELS,
+                   fused=bool(cfg.AMD.FUSED_BLOCKS))
 
 
 def assign_levels(boxes: torch.Tensor, min_level: int = 2, max_level: int = 5, canonical_size: float = 224.0, canonical_level: int = 4):

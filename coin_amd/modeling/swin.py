@@ -92,8 +92,12 @@ def shift_mask(hp: int, wp: int, ws: int, shift: int, device) -> torch.Tensor:
 
 
 class SwinBlock(nn.Module):
-    def __init__(self, dim: int, heads: int, window: int, shift: int, mlp_ratio: float = 4.0):
+    """``fused`` (cfg.AMD.FUSED_BLOCKS): on the device the norms and the residual add run on `L.residual_norm`, the linear layers with their
+    activation and residual on `L.fused_linear`; the same formulas, rounded in other places."""
+
+    def __init__(self, dim: int, heads: int, window: int, shift: int, mlp_ratio: float = 4.0, fused: bool = False):
         super().__init__()
+        self.fused = fused
         self.dim, self.heads, self.window, self.shift = dim, heads, window, shift
         self.norm1 = nn.LayerNorm(dim)
         self.qkv = nn.Linear(dim, dim * 3)
@@ -116,7 +120,9 @@ class SwinBlock(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:  # [N, H, W, C]
         n, h, w, c = x.shape
         ws, t = self.window, self.window * self.window
-        y = self.norm1(x)
+        fused = self.fused and x.is_cuda
+        linear = L.fused_linear if fused else L.linear
+        y = L.residual_norm(x, pre_norm=self.norm1)[1] if fused else self.norm1(x)
         ph, pw = (-h) % ws, (-w) % ws
         if ph or pw:
             y = F.pad(y, (0, 0, 0, pw, 0, ph))
@@ -125,16 +131,19 @@ class SwinBlock(nn.Module):
         if shift:
             y = torch.roll(y, shifts=(-shift, -shift), dims=(1, 2))
         win = y.view(n, hp // ws, ws, wp // ws, ws, c).permute(0, 1, 3, 2, 4, 5).reshape(-1, t, c)
-        qkv = L.linear(win, self.qkv.weight, self.qkv.bias)
+        qkv = linear(win, self.qkv.weight, self.qkv.bias)
         bias = self.relative_position_bias_table[self.relative_position_index.view(-1)].view(t, t, -1).permute(2, 0, 1)
         mask, mask64 = self._mask(hp, wp, x.device) if shift else (None, None)
         att = window_attention(qkv, bias, mask, mask64, self.heads, self.scale)
-        att = L.linear(att, self.proj.weight, self.proj.bias)
+        att = linear(att, self.proj.weight, self.proj.bias)
         y = att.view(n, hp // ws, wp // ws, ws, ws, c).permute(0, 1, 3, 2, 4, 5).reshape(n, hp, wp, c)
         if shift:
             y = torch.roll(y, shifts=(shift, shift), dims=(1, 2))
         if ph or pw:
             y = y[:, :h, :w, :]
+        if fused:
+            x, y = L.residual_norm(x, y, pre_norm=self.norm2)
+            return L.fused_linear(L.fused_linear(y, self.fc1.weight, self.fc1.bias, act=L.ACT_GELU), self.fc2.weight, self.fc2.bias, residual=x)
         x = x + y
         return x + L.linear(F.gelu(L.linear(self.norm2(x), self.fc1.weight, self.fc1.bias)), self.fc2.weight, self.fc2.bias)
 
@@ -154,14 +163,15 @@ class PatchMerging(nn.Module):
 
 
 class SwinTransformer(nn.Module):
-    def __init__(self, embed_dim: int = 96, depths=(2, 2, 6, 2), num_heads=(3, 6, 12, 24), window_size: int = 7, patch: int = 4):
+    def __init__(self, embed_dim: int = 96, depths=(2, 2, 6, 2), num_heads=(3, 6, 12, 24), window_size: int = 7, patch: int = 4,
+                 fused: bool = False):
         super().__init__()
         self.patch_embed = nn.Conv2d(3, embed_dim, patch, stride=patch)
         self.patch_norm = nn.LayerNorm(embed_dim)
         self.stages, self.merges, self.out_norms = nn.ModuleList(), nn.ModuleList(), nn.ModuleList()
         for i, (d, hds) in enumerate(zip(depths, num_heads)):
             dim = embed_dim * 2 ** i
-            self.stages.append(nn.Sequential(*[SwinBlock(dim, hds, window_size, 0 if k % 2 == 0 else window_size // 2) for k in range(d)]))
+            self.stages.append(nn.Sequential(*[SwinBlock(dim, hds, window_size, 0 if k % 2 == 0 else window_size // 2, fused=fused) for k in range(d)]))
             self.merges.append(PatchMerging(dim) if i < len(depths) - 1 else nn.Identity())
             self.out_norms.append(nn.LayerNorm(dim))
         self.patch = patch

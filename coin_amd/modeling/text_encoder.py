@@ -32,7 +32,7 @@ N_TEMPLATES = 81  # len(MODIFIED_REGION_CLIP_TEMPLATES), coin/modeling/utils.py:
 
 
 class _Attention(nn.Module):
-    """nn.MultiheadAttention parameter layout; causal self-attention via SDPA."""
+    """nn.MultiheadAttention parameter layout; causal self-attention via SDPA, or via `L.attention_qkv` in a fused block."""
 
     def __init__(self, d: int, heads: int):
         super().__init__()
@@ -49,24 +49,34 @@ class _Attention(nn.Module):
 
 
 class ResidualAttentionBlock(nn.Module):
-    def __init__(self, d: int, heads: int):
+    """``fused`` (cfg.AMD.FUSED_BLOCKS): on the device the block runs on `L.attention_qkv`, `L.residual_norm` and `L.fused_linear`; the same
+    formulas, rounded in other places."""
+
+    def __init__(self, d: int, heads: int, fused: bool = False):
         super().__init__()
+        self.fused = fused
         self.attn = _Attention(d, heads)
         self.ln_1 = nn.LayerNorm(d)
         self.mlp = nn.Sequential(OrderedDict([("c_fc", nn.Linear(d, d * 4)), ("gelu", nn.Identity()), ("c_proj", nn.Linear(d * 4, d))]))
         self.ln_2 = nn.LayerNorm(d)
 
     def forward(self, x):
+        if self.fused and x.is_cuda:
+            a, fc, pr = self.attn, self.mlp.c_fc, self.mlp.c_proj
+            _, h = L.residual_norm(x, pre_norm=self.ln_1)
+            y = L.attention_qkv(L.fused_linear(h, a.in_proj_weight, a.in_proj_bias), a.heads, causal=True)
+            x, h = L.residual_norm(x, L.fused_linear(y, a.out_proj.weight, a.out_proj.bias), pre_norm=self.ln_2)
+            return L.fused_linear(L.fused_linear(h, fc.weight, fc.bias, act=L.ACT_QUICK_GELU), pr.weight, pr.bias, residual=x)
         x = x + self.attn(self.ln_1(x))
         h = L.linear(self.ln_2(x), self.mlp.c_fc.weight, self.mlp.c_fc.bias)
         return x + L.linear(h * torch.sigmoid(1.702 * h), self.mlp.c_proj.weight, self.mlp.c_proj.bias)  # QuickGELU
 
 
 class Transformer(nn.Module):
-    def __init__(self, width: int, layers: int, heads: int):
+    def __init__(self, width: int, layers: int, heads: int, fused: bool = False):
         super().__init__()
         self.width, self.layers = width, layers
-        self.resblocks = nn.Sequential(*[ResidualAttentionBlock(width, heads) for _ in range(layers)])
+        self.resblocks = nn.Sequential(*[ResidualAttentionBlock(width, heads, fused) for _ in range(layers)])
 
     def forward(self, x):
         return self.resblocks(x)
@@ -85,10 +95,11 @@ def prompt_tokens(n_classes: int, context_length: int = 77, add_prompt_num: int 
 
 
 class TEXT_ENCODER(nn.Module):
-    def __init__(self, embed_dim, context_length, vocab_size, transformer_width, transformer_heads, transformer_layers, prompt_info):
+    def __init__(self, embed_dim, context_length, vocab_size, transformer_width, transformer_heads, transformer_layers, prompt_info,
+                 fused: bool = False):
         super().__init__()
         self.context_length = context_length
-        self.transformer = Transformer(transformer_width, transformer_layers, transformer_heads)
+        self.transformer = Transformer(transformer_width, transformer_layers, transformer_heads, fused)
         self.vocab_size = vocab_size
         self.token_embedding = nn.Embedding(vocab_size, transformer_width)
         self.positional_embedding = nn.Parameter(torch.empty(context_length, transformer_width))
@@ -234,12 +245,12 @@ class TEXT_ENCODER(nn.Module):
 class CLIP_TEXT(nn.Module):
     def __init__(self, type: str, classes: List[str], add_prompt_num: int = 4, dataset_style: str = "", embed_dim=None,
                  context_length=77, vocab_size=49408, width=512, heads=8, layers=12, tokenized_prompts=None,
-                 n_templates: int = N_TEMPLATES, graph: bool = True):
+                 n_templates: int = N_TEMPLATES, graph: bool = True, fused: bool = False):
         super().__init__()
         self.type, self.classes, self.dataset_style, self.add_prompt_num = type, list(classes), dataset_style, add_prompt_num
         embed_dim = embed_dim or TEXT_DIMS[type]
         toks = tokenized_prompts if tokenized_prompts is not None else prompt_tokens(len(classes), context_length, add_prompt_num, vocab_size=vocab_size)
-        self.encoder = TEXT_ENCODER(embed_dim, context_length, vocab_size, width, heads, layers, (toks, len(TEMPLATE_IDS), add_prompt_num))
+        self.encoder = TEXT_ENCODER(embed_dim, context_length, vocab_size, width, heads, layers, (toks, len(TEMPLATE_IDS), add_prompt_num), fused)
         self.encoder.use_graph = bool(graph)
         self.n_templates = n_templates
         self.load_embedding()
@@ -254,6 +265,7 @@ class CLIP_TEXT(nn.Module):
                    dataset_style=cfg.DATASETS.STYLE_NAME, n_templates=cfg.AMD.TEXT_TEMPLATES, embed_dim=a.TEXT_DIM or None,
                    context_length=a.CONTEXT_LENGTH, vocab_size=a.VOCAB_SIZE, width=a.TEXT_WIDTH or 512, heads=a.TEXT_HEADS or 8,
                    layers=a.TEXT_LAYERS or 12,
+                   fused=bool(getattr(cfg.AMD, "FUSED_BLOCKS", False)),
                    graph=bool(getattr(cfg.AMD, "TEXT_GRAPH", True)) and os.environ.get("COIN_TEXT_GRAPH", "1") != "0")
 
     @torch.no_grad()

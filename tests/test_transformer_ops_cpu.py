@@ -44,6 +44,17 @@ def test_attention_refusals(lib):
     assert lib.coin_attention_bwd(X, z, X, z, X, z, X, z, X, X, z, X, None, X, z, X, z, X, z, 1, 4, 4, 1, 1, 64, 0, 1.0, 1, None, 0, None) == -1        # no workspace
 
 
+def test_workspace_queries_take_empty_shapes(lib):
+    for b in (0, 1, 3):
+        for lq in (0, 1, 5000):
+            for lk in (0, 1, 5000):
+                for back in (0, 1):
+                    n = lib.coin_attention_workspace_bytes(b, lq, lk, 4, 2, 64, 1, back)
+                    assert (n == 0) if b == 0 else n >= 0
+    assert lib.coin_linear_workspace_bytes(0, 8, 8, 1, 0) == 0 and lib.coin_linear_workspace_bytes(0, 8, 8, 0, 1) == 0
+    assert lib.coin_linear_workspace_bytes(1, 1, 1, 1, 1) > 0 and lib.coin_residual_norm_bwd_workspace_bytes(1, 1) > 0
+
+
 def norm(lib, x=X, y=X, gate=None, group=8, post=0, pre=1, r=X, h=X, stats=None, m=8, d=16, ts=0, tb=0, tg=0):
     return lib.coin_residual_norm_fwd(x, y, gate, group, None, None, post, 1e-5, None, None, pre, 1e-5, 0, 1.0, r, h, stats, m, d, ts, tb, tg, None)
 
