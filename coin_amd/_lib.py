@@ -99,8 +99,7 @@ SIGNATURES = {
     "coin_residual_norm_bwd": [_P, _P, _P, _L, _P, _P, _I, _P, _I, _I, _F] + [_P] * 10 + [_L, _I, _I, _I, _I, _P, _Z, _P],
     "coin_linear_workspace_bytes": [_L, _I, _I, _I, _I],
     "coin_linear_fwd": [_P, _L, _P, _L, _P, _I, _I, _P, _L, _P, _L, _I, _P, _L, _L, _I, _I, _I, _P, _Z, _P],
-    "coin_linear_dz": [_P, _L, _I, _P, _L, _P, _L, _P, _I, _L, _I, _I, _P, _Z, _P],
-    "coin_linear_bwd": [_P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _I, _L, _I, _I, _I, _P, _Z, _P],
+    "coin_linear_bwd": [_P, _L, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _I, _P, _I, _L, _I, _I, _I, _P, _Z, _P],
     "coin_pad_rows": [_P, _L, _P, _L, _L, _I, _I, _P],
 }
 

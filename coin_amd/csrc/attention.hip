@@ -161,7 +161,9 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
   f32x16 o[C::ND];
 #pragma unroll
   for (int d = 0; d < C::ND; ++d) o[d] = zero16();
-  float m = -INFINITY, l = 0.f;
+  // l: the sum that L is made of.  lw: the sum of the rounded probabilities that the product takes; o = sum p~ v / sum p~ is off by the
+  // roundings times (v_j - o) instead of v_j, which is what D and through it dQ and dK see
+  float m = -INFINITY, l = 0.f, lw = 0.f;
   const float c = p.c;
   if (kb < ke) stage(kb, 0);
   int buf = 0;
@@ -196,31 +198,38 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
       const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
       m = mn;
       l *= al;
+      lw *= al;
 #pragma unroll
       for (int d = 0; d < C::ND; ++d) o[d] *= al;
     }
     const float mc = m == -INFINITY ? 0.f : m * c;
-    float ls = 0.f;
+    float ls = 0.f, lr = 0.f;
 #pragma unroll
     for (int s = 0; s < C::NS; ++s)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         st[s][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[s][r], c, -mc));
         ls += st[s][r];
+        if constexpr (sizeof(T) == 2) {
+          st[s][r] = (float)(bf16_t)st[s][r];
+          lr += st[s][r];
+        }
       }
     l += ls;
+    if (sizeof(T) == 2) lw += lr;
 #pragma unroll
     for (int s = 0; s < C::NS; ++s)
       if (sizeof(T) == 2 || kt + s * 32 < wmax) mma_t<T, I, C::ND>(o, vimg, s * 32, st[s], lane);
   }
   l += __shfl_xor(l, 32, 64);
+  lw += __shfl_xor(lw, 32, 64);
+  if (sizeof(T) == 4) lw = l;
   if (!live) return;
   const size_t row = (size_t)bh * p.R + t;
   if (SPLIT) {   // unnormalised sums with their maximum; joined by attention_join_kernel.  A split without keys leaves l = 0 and no sums
     const size_t prow = (size_t)split * nbh * p.R + row;
     if (half == 0) {
-      p.part_ml[prow * 2] = m == -INFINITY ? 0.f : m * c;
-      p.part_ml[prow * 2 + 1] = l;
+      *reinterpret_cast<f32x4*>(p.part_ml + prow * 4) = (f32x4){m == -INFINITY ? 0.f : m * c, l, lw, 0.f};
     }
     if (kb < wmax && l > 0.f) {
 #pragma unroll
@@ -233,7 +242,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
     }
     return;
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // no key: zeros; NaN stays
+  const float inv = lw > 0.f ? 1.f / lw : (lw == 0.f ? 0.f : lw);   // no key: zeros; NaN stays
   if (p.lse && half == 0) p.lse[row] = l == 0.f ? INFINITY : m * c + __builtin_amdgcn_logf(l);
   T* op = (T*)p.out + b * p.os[0] + (int64_t)i * p.os[1] + (int64_t)(hk * p.g + gi) * p.os[2];
   bf16_t* lp = p.lo ? p.lo + (((size_t)b * p.Lq + i) * p.Hkv * p.g + hk * p.g + gi) * p.D : nullptr;
@@ -265,24 +274,26 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
   float m = -INFINITY;
   bool bad = false;
   for (int s = lane; s < p.splits; s += 64) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + row) * 2);
-    if (ml.y != 0.f) m = fmaxf(m, ml.x);
-    bad |= !(ml.y == ml.y);
+    const f32x4 ml = *reinterpret_cast<const f32x4*>(p.part_ml + (s * rows + row) * 4);
+    if (ml[1] != 0.f) m = fmaxf(m, ml[0]);
+    bad |= !(ml[1] == ml[1]);
   }
   m = wave_reduce_max(m);
   bad = __any(bad);
-  float a0 = 0.f, a1 = 0.f, l = 0.f;
+  float a0 = 0.f, a1 = 0.f, l = 0.f, lw = 0.f;
   const int d = lane * 2;   // head dimensions are even and <= 128
   for (int s0 = 0; s0 < p.splits; s0 += 64) {
-    float w = 0.f, ls = 0.f;
+    float w = 0.f, ls = 0.f, lr = 0.f;
     if (s0 + lane < p.splits) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((s0 + lane) * rows + row) * 2);
-      if (ml.y > 0.f) {
-        w = __builtin_amdgcn_exp2f(ml.x - m);
-        ls = ml.y * w;
+      const f32x4 ml = *reinterpret_cast<const f32x4*>(p.part_ml + ((s0 + lane) * rows + row) * 4);
+      if (ml[1] > 0.f) {
+        w = __builtin_amdgcn_exp2f(ml[0] - m);
+        ls = ml[1] * w;
+        lr = ml[2] * w;
       }
     }
     l += wave_reduce_sum(ls);
+    lw += wave_reduce_sum(lr);
     const int ns = p.splits - s0 < 64 ? p.splits - s0 : 64;
 #pragma unroll 8
     for (int s = 0; s < ns; ++s) {
@@ -293,8 +304,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
       a1 = __builtin_fmaf(v.y, ws, a1);
     }
   }
-  if (bad) l = __builtin_nanf("");
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (bad) l = lw = __builtin_nanf("");
+  const float inv = lw == 0.f ? 0.f : 1.f / lw;
   const int bh = (int)(row / p.R), t = (int)(row - (int64_t)bh * p.R), b = bh / p.Hkv, hk = bh - b * p.Hkv, i = t / p.g, gi = t - i * p.g;
   if (p.lse && lane == 0) p.lse[row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
   if (d < p.D) {
@@ -647,7 +658,7 @@ static Plan make_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv
   p.fw = fwd_waves(R, nbh);
   p.fsplits = p.fw == 1 ? fwd_splits((R + 31) / 32 * nbh, (int)Lk, &p.fchunk) : 1;
   if (p.fsplits == 1) p.fchunk = (int)Lk;
-  p.fwd_bytes = p.fsplits > 1 ? (size_t)p.fsplits * nbh * R * (D + 2) * sizeof(float) : 0;
+  p.fwd_bytes = p.fsplits > 1 ? (size_t)p.fsplits * nbh * R * (D + 4) * sizeof(float) : 0;
   p.kw = dkv_waves(Lk, nbh);
   p.ksplits = dkv_splits((Lk + p.kw * 32 - 1) / (p.kw * 32) * nbh, R);
   p.bwd_bytes = (size_t)nbh * R * sizeof(float);

@@ -681,15 +681,24 @@ extern "C" int coin_pad_rows(const void* src, int64_t ld_src, void* dst, int64_t
   return coin_launch_status();
 }
 
+static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+static size_t dz_bytes(int64_t M, int N, int es) { return up256((size_t)M * ((N + 7) / 8 * 8) * es); }
+
+// what the products and the column sums of a backward share, one after the other
+static size_t bwd_part_bytes(int64_t M, int N, int K, int es) {
+  int rows;
+  size_t n = (size_t)dz_blocks(M, N, &rows) * N * sizeof(float);
+  const size_t a = part_bytes(M, K, N, es), b = part_bytes(N, K, M, es);
+  n = a > n ? a : n;
+  return b > n ? b : n;
+}
+
 extern "C" size_t coin_linear_workspace_bytes(int64_t M, int N, int K, int dtype, int backward) {
   if (check_lin(M, N, K, dtype) != COIN_OK || M == 0) return 0;
   const int es = dtype == COIN_BF16 ? 2 : 4;
   if (!backward) return part_bytes(M, N, K, es);
-  size_t a = part_bytes(M, K, N, es), b = part_bytes(N, K, M, es);
-  int rows;
-  const size_t c = (size_t)dz_blocks(M, N, &rows) * N * sizeof(float);
-  if (b > a) a = b;
-  return a > c ? a : c;
+  return (backward > 1 ? dz_bytes(M, N, es) : 0) + bwd_part_bytes(M, N, K, es);
 }
 
 extern "C" int coin_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int act, const void* residual,
@@ -716,57 +725,45 @@ extern "C" int coin_linear_fwd(const void* x, int64_t ldx, const void* w, int64_
   return coin_launch_status();
 }
 
-extern "C" int coin_linear_dz(const void* dy, int64_t ldy, int dy_dtype, const void* slope, int64_t ld_slope, void* dz, int64_t ldz, void* db, int db_dtype,
-                              int64_t M, int N, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-  int rc = check_lin(M, N, 1, dtype);
-  if (rc != COIN_OK) return rc;
-  if (!dy || (!dz && !db) || M == 0 || (dy_dtype != COIN_F32 && dy_dtype != COIN_BF16) || (dtype == COIN_F32 && dy_dtype != COIN_F32)) return COIN_EINVAL;
-  if (db && db_dtype != COIN_F32 && db_dtype != COIN_BF16) return COIN_EINVAL;
-  if (ldy < N || (slope && ld_slope < N)) return COIN_EINVAL;
-  if (dz && (!al16(dz) || ldz % 8 || ldz < (N + 7) / 8 * 8)) return COIN_EALIGN;
-  DzArgs a = {};
-  a.dy = dy; a.ldy = ldy; a.dy_f32 = dy_dtype == COIN_F32; a.slope = slope; a.lds_ = ld_slope; a.dz = dz; a.ldz = ldz; a.M = M; a.N = N;
-  a.vec = N % 8 == 0 && ldy % 8 == 0 && al16(dy) && (!slope || (ld_slope % 8 == 0 && al16(slope)));
-  const int blocks = dz_blocks(M, N, &a.rows);
-  if (db) {
-    if (!workspace || workspace_bytes < (size_t)blocks * N * sizeof(float)) return COIN_EINVAL;
-    a.part = (float*)workspace;
-  }
-  hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((N + 255) / 256, blocks);
-  if (dtype == COIN_BF16) linear_dz_kernel<bf16_t><<<grid, 256, 0, st>>>(a);
-  else linear_dz_kernel<float><<<grid, 256, 0, st>>>(a);
-  if (db) linear_db_kernel<<<(N + 63) / 64, 256, 0, st>>>(a.part, db, db_dtype == COIN_F32, blocks, N);
-  return coin_launch_status();
-}
-
-extern "C" int coin_linear_bwd(const void* dz, int64_t ldz, const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx, int64_t lddx, void* dw,
-                               int64_t lddw, int dw_dtype, int64_t M, int N, int K, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int coin_linear_bwd(const void* dy, int64_t ldy, int dy_dtype, const void* slope, int64_t ld_slope, const void* x, int64_t ldx, const void* w,
+                               int64_t ldw, void* dx, int64_t lddx, void* dw, int64_t lddw, int dw_dtype, void* db, int db_dtype, int64_t M, int N, int K,
+                               int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_lin(M, N, K, dtype);
   if (rc != COIN_OK) return rc;
-  if ((!dx && !dw) || M == 0) return COIN_EINVAL;
+  if (!dy || (!dx && !dw && !db) || M == 0 || ldy < N || (slope && ld_slope < N)) return COIN_EINVAL;
+  if ((dy_dtype != COIN_F32 && dy_dtype != COIN_BF16) || (dtype == COIN_F32 && dy_dtype != COIN_F32)) return COIN_EINVAL;
+  if (db && db_dtype != COIN_F32 && db_dtype != COIN_BF16) return COIN_EINVAL;
   if (dw && dw_dtype != COIN_F32 && (dw_dtype != COIN_BF16 || dtype == COIN_F32)) return COIN_EINVAL;
+  if ((dx && lddx < K) || (dw && lddw < K)) return COIN_EINVAL;
   const int es = dtype == COIN_BF16 ? 2 : 4;
-  if ((rc = check_op(dz, ldz, N, es)) != COIN_OK) return rc;
-  if (workspace && !al16(workspace)) return COIN_EALIGN;
+  if (dx && (rc = check_op(w, ldw, K, es)) != COIN_OK) return rc;
+  if (dw && (rc = check_op(x, ldx, K, es)) != COIN_OK) return rc;
+  // dz is dy itself where there is no activation, its type is the products' and its rows are whole chunks
+  const bool products = dx || dw;
+  const bool own = products && (slope || dy_dtype != dtype || N % (16 / es) || check_op(dy, ldy, N, es) != COIN_OK);
+  if (!workspace || workspace_bytes < (own ? dz_bytes(M, N, es) : 0) + bwd_part_bytes(M, N, K, es)) return COIN_EINVAL;
+  if (!al16(workspace)) return COIN_EALIGN;
   hipStream_t st = (hipStream_t)stream;
-  if (dx) {
-    if (lddx < K) return COIN_EINVAL;
-    if ((rc = check_op(w, ldw, K, es)) != COIN_OK) return rc;
-    const size_t need = part_bytes(M, K, N, es);
-    if (need && (!workspace || workspace_bytes < need)) return COIN_EINVAL;
-  }
-  if (dw) {
-    if (lddw < K) return COIN_EINVAL;
-    if ((rc = check_op(x, ldx, K, es)) != COIN_OK) return rc;
-    const size_t need = part_bytes(N, K, M, es);
-    if (need && (!workspace || workspace_bytes < need)) return COIN_EINVAL;
+  float* part = (float*)((char*)workspace + (own ? dz_bytes(M, N, es) : 0));
+  const void* dz = own ? workspace : dy;
+  const int64_t ldz = own ? (N + 7) / 8 * 8 : ldy;
+  if (products && (rc = check_op(dz, ldz, N, es)) != COIN_OK) return rc;
+  if (own || db) {
+    DzArgs a = {};
+    a.dy = dy; a.ldy = ldy; a.dy_f32 = dy_dtype == COIN_F32; a.slope = slope; a.lds_ = ld_slope; a.dz = own ? workspace : nullptr; a.ldz = ldz;
+    a.M = M; a.N = N; a.part = db ? part : nullptr;
+    a.vec = N % 8 == 0 && ldy % 8 == 0 && al16(dy) && (!slope || (ld_slope % 8 == 0 && al16(slope)));
+    const int blocks = dz_blocks(M, N, &a.rows);
+    const dim3 grid((N + 255) / 256, blocks);
+    if (dtype == COIN_BF16) linear_dz_kernel<bf16_t><<<grid, 256, 0, st>>>(a);
+    else linear_dz_kernel<float><<<grid, 256, 0, st>>>(a);
+    if (db) linear_db_kernel<<<(N + 63) / 64, 256, 0, st>>>(part, db, db_dtype == COIN_F32, blocks, N);
   }
   if (dx) {
     LinArgs a = {};
     a.A = dz; a.lda = ldz; a.B = w; a.ldb = ldw; a.M = (int)M; a.N = K; a.K = N; a.C = dx; a.ldc = lddx; a.c_f32 = dtype == COIN_F32;
     a.vec = K % 8 == 0 && lddx % 8 == 0 && al16(dx);
-    a.part = (float*)workspace;
+    a.part = part;
     if (dtype == COIN_BF16) run_gemm<bf16_t, false, true>(a, st);
     else run_gemm<float, false, true>(a, st);
   }
@@ -774,7 +771,7 @@ extern "C" int coin_linear_bwd(const void* dz, int64_t ldz, const void* x, int64
     LinArgs a = {};
     a.A = dz; a.lda = ldz; a.B = x; a.ldb = ldx; a.M = N; a.N = K; a.K = (int)M; a.C = dw; a.ldc = lddw; a.c_f32 = dw_dtype == COIN_F32;
     a.vec = K % 8 == 0 && lddw % 8 == 0 && al16(dw);
-    a.part = (float*)workspace;
+    a.part = part;
     if (dtype == COIN_BF16) run_gemm<bf16_t, true, true>(a, st);
     else run_gemm<float, true, true>(a, st);
   }

@@ -18,7 +18,7 @@ from ._lib import ACT_LEAKY_RELU, ACT_NONE, ACT_RELU, COIN_BF16, COIN_F32, COIN_
 __all__ = [
     "roi_align_fwd", "roi_align_bwd", "gemm_nt", "conv_gemm", "conv_wgrad", "window_attn_fwd", "window_attn_bwd", "roi_align_fwd_levels", "roi_align_bwd_level", "conv_stats_finalize", "transpose2d", "bias_act_bwd", "cosine_logits_fwd",
     "cosine_logits_bwd", "bn_stats", "bn_apply_fwd", "bn_bwd", "avgpool2_fwd", "avgpool2_bwd", "nms_batched", "mil_ce", "mil_focal", "kl_div", "box_reg_l1", "l1_mean", "rpn_losses", "normalize_pad",
-    "SgdTable", "EmaTable", "attention_plan", "attention_fwd", "attention_bwd", "residual_norm_fwd", "residual_norm_bwd", "chunked_rows", "linear_fwd", "linear_dz", "linear_bwd",
+    "SgdTable", "EmaTable", "attention_plan", "attention_fwd", "attention_bwd", "residual_norm_fwd", "residual_norm_bwd", "chunked_rows", "linear_fwd", "linear_bwd",
 ]
 
 
@@ -1195,29 +1195,20 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, k: int, bias: Optional[torch.Te
     return y, slope
 
 
-def linear_dz(dy: torch.Tensor, slope: Optional[torch.Tensor], dtype: torch.dtype, want_dz: bool, db_dtype: Optional[torch.dtype]):
-    """coin_linear_dz: dz = dy o slope as rows for `linear_bwd`, and its column sums -> (dz or None, db or None)."""
-    m, n = dy.shape
-    index = _device_of(dy, slope)
+def linear_bwd(dy: torch.Tensor, slope: Optional[torch.Tensor], x: Optional[torch.Tensor], w: Optional[torch.Tensor], n: int, k: int, dtype: torch.dtype,
+               want_dx: bool, dw_dtype: Optional[torch.dtype], db_dtype: Optional[torch.dtype]):
+    """coin_linear_bwd from dy [M, n] rows and `linear_fwd`'s slope -> (dx [M, k] or None, dW [n, k] or None, db [n] or None); x serves dW and w
+    dx, both as `linear_fwd` took them."""
+    m = dy.shape[0]
+    index = _device_of(dy, slope, x, w)
     dev, code = dy.device, _code(dtype)
-    dz = torch.empty((m, (n + 7) // 8 * 8), dtype=dtype, device=dev) if want_dz else None
-    db = torch.empty(n, dtype=db_dtype, device=dev) if db_dtype is not None else None
-    nbytes = _linear_ws(m, n, 1, code, 1) if db is not None else 0
-    ws = _workspace(nbytes, dev)
-    _launch(index, "coin_linear_dz", dy.data_ptr(), _pitch(dy), _code(dy.dtype), _a(slope), slope.shape[1] if slope is not None else 0, _a(dz),
-            dz.shape[1] if want_dz else 0, _a(db), _code(db_dtype) if db is not None else COIN_F32, m, n, code, _a(ws), nbytes)
-    return dz, db
-
-
-def linear_bwd(dz: torch.Tensor, x: Optional[torch.Tensor], w: Optional[torch.Tensor], n: int, k: int, want_dx: bool, dw_dtype: Optional[torch.dtype]):
-    """coin_linear_bwd on `chunked_rows` operands -> (dx [M, k] or None, dW [n, k] or None); x serves dW, w serves dx."""
-    m = dz.shape[0]
-    index = _device_of(dz, x, w)
-    dev, code = dz.device, _code(dz.dtype)
-    dx = torch.empty((m, k), dtype=dz.dtype, device=dev) if want_dx else None
+    dx = torch.empty((m, k), dtype=dtype, device=dev) if want_dx else None
     dw = torch.empty((n, k), dtype=dw_dtype, device=dev) if dw_dtype is not None else None
-    nbytes = _linear_ws(m, n, k, code, 1)
+    db = torch.empty(n, dtype=db_dtype, device=dev) if db_dtype is not None else None
+    as_is = slope is None and dy.dtype == dtype and chunked_ok(dy)
+    nbytes = _linear_ws(m, n, k, code, 1 if as_is or (dx is None and dw is None) else 2)
     ws = _workspace(nbytes, dev)
-    _launch(index, "coin_linear_bwd", dz.data_ptr(), _pitch(dz), _a(x), _pitch(x), _a(w), _pitch(w), _a(dx), k, _a(dw), k,
-            _code(dw_dtype) if dw is not None else COIN_F32, m, n, k, code, _a(ws), nbytes)
-    return dx, dw
+    _launch(index, "coin_linear_bwd", dy.data_ptr(), _pitch(dy), _code(dy.dtype), _a(slope), slope.shape[1] if slope is not None else 0, _a(x), _pitch(x),
+            _a(w), _pitch(w), _a(dx), k, _a(dw), k, _code(dw_dtype) if dw is not None else COIN_F32, _a(db),
+            _code(db_dtype) if db is not None else COIN_F32, m, n, k, code, _a(ws), nbytes)
+    return dx, dw, db

@@ -1109,16 +1109,10 @@ class _FusedLinear(Function):
         need_x, need_w, need_b, need_res, _, _ = ctx.needs_input_grad
         dx = dw = db = None
         if need_x or need_w or need_b:
-            products = need_x or need_w
-            g = _rows(dy)
-            as_is = products and slope is None and g.dtype == ctx.dtype and K.chunked_ok(g)   # dz is dy
-            dz = g
-            if not as_is or need_b:
-                dz, db = K.linear_dz(g, slope, ctx.dtype, products and not as_is, ctx.db_dtype if need_b else None)
-            if products:
-                dx, dw = K.linear_bwd(g if as_is else dz, xr, wr, ctx.n, ctx.k, need_x, ctx.dw_dtype if need_w else None)
-                if need_x and len(ctx.shape) != 2:
-                    dx = dx.view(ctx.shape)
+            dx, dw, db = K.linear_bwd(_rows(dy), slope, xr, wr, ctx.n, ctx.k, ctx.dtype, need_x, ctx.dw_dtype if need_w else None,
+                                      ctx.db_dtype if need_b else None)
+            if need_x and len(ctx.shape) != 2:
+                dx = dx.view(ctx.shape)
         return dx, dw, db, (dy if need_res else None), None, None
 
 

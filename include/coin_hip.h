@@ -510,19 +510,19 @@ int coin_residual_norm_bwd(const void* x, const void* y, const void* gate, int64
  * act NONE, RELU, GELU, QUICK_GELU or SILU.  slope (NULL when no backward follows): act'(z) [M][ld_slope], half precision for bfloat16
  * layers, float32 for float32 ones.
  * x and W rows: 16-byte aligned, leading dimensions of whole 16-byte chunks that hold the row's last chunk whole (COIN_EALIGN; coin_pad_rows
- * makes such rows); where K is not a multiple of a chunk (8 bf16, 4 f32) the rest of the last chunk holds ZEROS.  The same for dz below.
+ * makes such rows); where K is not a multiple of a chunk (8 bf16, 4 f32) the rest of the last chunk holds ZEROS.
  * 260 rows' span below 2^31 bytes (COIN_ESHAPE).  workspace: coin_linear_workspace_bytes, 16-byte aligned. */
 size_t coin_linear_workspace_bytes(int64_t M, int N, int K, int dtype, int backward);
 int coin_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int act, const void* residual,
                     int64_t ldr, void* y, int64_t ldy, int y_dtype, void* slope, int64_t ld_slope, int64_t M, int N, int K, int dtype,
                     void* workspace, size_t workspace_bytes, void* stream);
-/* dz = dy o slope (slope NULL: dy) in `dtype`, rows of ldz elements (a multiple of 8) with zeros in the rest of the last chunk, and/or
- * db = column sums of dz before its rounding.  dz or db may be NULL.  M > 0. */
-int coin_linear_dz(const void* dy, int64_t ldy, int dy_dtype, const void* slope, int64_t ld_slope, void* dz, int64_t ldz, void* db, int db_dtype,
-                   int64_t M, int N, int dtype, void* workspace, size_t workspace_bytes, void* stream);
-/* dx [M][K] = dz W of `dtype` and / or dw [N][K] = dz^T x of dw_dtype (float32 layers: float32).  M > 0. */
-int coin_linear_bwd(const void* dz, int64_t ldz, const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx, int64_t lddx, void* dw,
-                    int64_t lddw, int dw_dtype, int64_t M, int N, int K, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+/* Its backward from dy [M][N] (dy_dtype, any pitch and alignment) and the forward's slope (NULL: no activation): dz = dy o slope,
+ * dx [M][K] = dz W of `dtype`, dw [N][K] = dz^T x of dw_dtype (float32 layers: float32), db [N] = column sums of dz before its rounding, of
+ * db_dtype; each OVERWRITTEN or NULL where it is not wanted.  M > 0.  workspace: coin_linear_workspace_bytes with backward = 2; backward = 1 is
+ * enough where dz is dy itself: no slope, dy of `dtype` in rows as x's. */
+int coin_linear_bwd(const void* dy, int64_t ldy, int dy_dtype, const void* slope, int64_t ld_slope, const void* x, int64_t ldx, const void* w,
+                    int64_t ldw, void* dx, int64_t lddx, void* dw, int64_t lddw, int dw_dtype, void* db, int db_dtype, int64_t M, int N, int K,
+                    int dtype, void* workspace, size_t workspace_bytes, void* stream);
 /* dst [rows][ld_dst] = src [rows][cols] (row pitch ld_src) with zeros behind the columns; ld_dst a multiple of 8. */
 int coin_pad_rows(const void* src, int64_t ld_src, void* dst, int64_t ld_dst, int64_t rows, int cols, int dtype, void* stream);
 

@@ -82,13 +82,15 @@ def test_linear_refusals(lib):
     need = lib.coin_linear_workspace_bytes(4, 64, 8192, 1, 0)
     assert need > 0 and fwd(m=4, n=64, ldy=64, k=8192, ldx=8192, ldw=8192) == -1
     assert fwd(m=4, n=64, ldy=64, k=8192, ldx=8192, ldw=8192, ws=X, nb=need - 1) == -1 and fwd(m=4, n=64, ldy=64, k=8192, ldx=8192, ldw=8192, ws=ODD, nb=need) == -3
-    assert lib.coin_linear_dz(X, 32, 1, None, 0, None, 0, None, 0, 8, 32, 1, None, 0, None) == -1      # neither dz nor db
-    assert lib.coin_linear_dz(X, 32, 1, None, 0, X, 33, None, 0, 8, 32, 1, None, 0, None) == -3
-    assert lib.coin_linear_dz(X, 32, 1, None, 0, None, 0, X, 0, 8, 32, 1, None, 0, None) == -1         # db without its workspace
-    assert lib.coin_linear_bwd(X, 32, X, 64, X, 64, None, 0, None, 0, 0, 8, 32, 64, 1, None, 0, None) == -1
-    assert lib.coin_linear_bwd(X, 32, X, 64, X, 64, X, 63, None, 0, 0, 8, 32, 64, 1, None, 0, None) == -1
-    assert lib.coin_linear_bwd(X, 30, X, 64, X, 64, X, 64, None, 0, 0, 8, 32, 64, 1, None, 0, None) == -3
-    assert lib.coin_linear_bwd(X, 32, X, 64, X, 64, None, 0, X, 64, 1, 8, 32, 64, 0, None, 0, None) == -1   # float32 layer, bfloat16 dW
+    full = lib.coin_linear_workspace_bytes(8, 32, 64, 1, 2)
+    bwd = lambda dy=X, ldy=32, ty=1, slope=None, lds=0, x=X, ldx=64, w=X, ldw=64, dx=None, lddx=64, dw=None, lddw=64, tw=0, db=None, tb=0, m=8, n=32, dt=1, ws=X, nb=full: (  # noqa: E731
+        lib.coin_linear_bwd(dy, ldy, ty, slope, lds, x, ldx, w, ldw, dx, lddx, dw, lddw, tw, db, tb, m, n, 64, dt, ws, nb, None))
+    assert full > lib.coin_linear_workspace_bytes(8, 32, 64, 1, 1) > 0
+    assert bwd() == -1 and bwd(dy=None, dx=X) == -1 and bwd(dx=X, m=0) == -1 and bwd(dx=X, ldy=31) == -1 and bwd(dx=X, slope=X, lds=31) == -1
+    assert bwd(dx=X, lddx=63) == -1 and bwd(dw=X, lddw=63) == -1 and bwd(db=X, tb=3) == -1 and bwd(dx=X, ty=0, dt=0, ws=None) == -1
+    assert bwd(dw=X, tw=1, dt=0, ty=0) == -1 and bwd(dx=X, dt=0, ty=1) == -1             # a float32 layer has float32 gradients
+    assert bwd(dx=X, w=None) == -1 and bwd(dx=X, w=ODD) == -3 and bwd(dw=X, ldx=60) == -3 and bwd(dw=X, x=None) == -1
+    assert bwd(dx=X, slope=X, lds=32, nb=full - 1) == -1 and bwd(dx=X, ws=ODD) == -3 and bwd(db=X, ws=None) == -1
     assert lib.coin_pad_rows(X, 5, X, 12, 4, 5, 1, None) == -2 and lib.coin_pad_rows(X, 5, X, 4, 4, 5, 1, None) == -1 and lib.coin_pad_rows(X, 5, X, 8, 0, 5, 1, None) == 0
 
 
