@@ -34,36 +34,26 @@ struct LinArgs {
   int tiles_m, tiles_n;
 };
 
-// Phi(z) and exp(-z^2 / 2).  bfloat16 layers: Abramowitz & Stegun 7.1.26 (erfc x = exp(-x^2) P(t), t = 1 / (1 + p x), absolute error
-// 1.5e-7), which shares its exponential with the slope: 18 instructions an element where the library's erfc and exp take 80, and those 80
-// were 0.25 ms of 0.93 ms on [16381 x 8192] outputs.
-template <typename T>
+// Phi(z) and exp(-z^2 / 2) by Abramowitz & Stegun 7.1.26 (erfc x = exp(-x^2) P(t), t = 1 / (1 + p x), absolute error 1.5e-7: a float32 product
+// of a few hundred terms is off by as much), which shares its exponential with the slope: 18 instructions a value where the library's erfc and
+// exp take 80, and those 80 were 0.25 ms of 0.93 ms on [16381 x 8192] outputs
 __device__ __forceinline__ void normal_cdf(float z, float& cdf, float& bell) {
-  if constexpr (sizeof(T) == 4) {
-    cdf = 0.5f * erfcf(z * -0.70710678118654752f);
-    bell = expf(-0.5f * z * z);
-  } else {
-    const float x = fabsf(z) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
-    float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-    q = __builtin_fmaf(q, t, 1.421413741f);
-    q = __builtin_fmaf(q, t, -0.284496736f);
-    q = __builtin_fmaf(q, t, 0.254829592f);
-    bell = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
-    q = 0.5f * q * t * bell;   // Phi(-|z|)
-    cdf = z < 0.f ? q : 1.f - q;
-  }
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+  float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  q = __builtin_fmaf(q, t, 1.421413741f);
+  q = __builtin_fmaf(q, t, -0.284496736f);
+  q = __builtin_fmaf(q, t, 0.254829592f);
+  bell = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+  q = 0.5f * q * t * bell;   // Phi(-|z|)
+  cdf = z < 0.f ? q : 1.f - q;
 }
 
-template <typename T>
-__device__ __forceinline__ float sigmoid_of(float x) {
-  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-x));
-  else return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
-}
+__device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f)); }
 
 // v <- act(v) for eight values, and act'(v) into sl where SLOPE.  The activation is chosen once for the eight: a choice per value made the
 // epilogue's code larger than the instruction cache
-template <typename T, bool SLOPE>
+template <bool SLOPE>
 __device__ __forceinline__ void act8(float (&v)[8], float (&sl)[8], int act) {
   if (act == COIN_ACT_NONE) {
 #pragma unroll
@@ -78,7 +68,7 @@ __device__ __forceinline__ void act8(float (&v)[8], float (&sl)[8], int act) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float cdf, bell;
-      normal_cdf<T>(v[i], cdf, bell);
+      normal_cdf(v[i], cdf, bell);
       if (SLOPE) sl[i] = __builtin_fmaf(v[i] * 0.39894228040143268f, bell, cdf);
       v[i] *= cdf;
     }
@@ -86,7 +76,7 @@ __device__ __forceinline__ void act8(float (&v)[8], float (&sl)[8], int act) {
     const float a = act == COIN_ACT_QUICK_GELU ? 1.702f : 1.f;   // z sigmoid(a z)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float s = sigmoid_of<T>(a * v[i]);
+      const float s = sigmoid_of(a * v[i]);
       if (SLOPE) sl[i] = s * (1.f + a * v[i] * (1.f - s));
       v[i] *= s;
     }
@@ -134,8 +124,8 @@ __device__ __forceinline__ void finish8(const LinArgs& p, float (&v)[8], const f
   if (p.res) residual8(p, r, ahead, row, col);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] += bias[i];
-  if (p.slope) act8<T, true>(v, sl, p.act);
-  else act8<T, false>(v, sl, p.act);
+  if (p.slope) act8<true>(v, sl, p.act);
+  else act8<false>(v, sl, p.act);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] += r[i];
   if (p.vec) {
