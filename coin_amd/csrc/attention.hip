@@ -683,7 +683,7 @@ static int check_tensor(const void* p, const int64_t* s, int es, int64_t g) {
   if ((uintptr_t)p & 15) return COIN_EALIGN;
   for (int i = 0; i < 3; ++i)
     if (s[i] < 0 || (s[i] * es) & 15) return COIN_EALIGN;
-  if (s[1] >= SPAN || s[2] >= SPAN || 66 * s[1] * es + g * s[2] * es >= SPAN) return COIN_ESHAPE;
+  if (s[1] >= SPAN || s[2] >= SPAN || 130 * s[1] * es + g * s[2] * es >= SPAN) return COIN_ESHAPE;
   return COIN_OK;
 }
 
@@ -747,7 +747,7 @@ extern "C" int coin_attention_fwd(const void* q, const int64_t* q_strides, const
                                   int D, int causal, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_shape(B, Lq, Lk, Hq, Hkv, D, dtype);
   if (rc != COIN_OK) return rc;
-  if (!(scale > 0.f) || scale > 3.0e38f) return COIN_EINVAL;
+  if (!(scale > 0.f) || scale > 1.0e30f) return COIN_EINVAL;
   if (B == 0 || Lq == 0) return COIN_OK;
   const int es = dtype == COIN_BF16 ? 2 : 4, g = Hq / Hkv;
   if ((rc = check_tensor(q, q_strides, es, g)) != COIN_OK || (rc = check_tensor(out, out_strides, es, g)) != COIN_OK) return rc;
@@ -776,7 +776,7 @@ extern "C" int coin_attention_bwd(const void* q, const int64_t* q_strides, const
                                   void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_shape(B, Lq, Lk, Hq, Hkv, D, dtype);
   if (rc != COIN_OK) return rc;
-  if (!(scale > 0.f) || scale > 3.0e38f) return COIN_EINVAL;
+  if (!(scale > 0.f) || scale > 1.0e30f) return COIN_EINVAL;
   if (B == 0 || (Lq == 0 && Lk == 0)) return COIN_OK;
   const int es = dtype == COIN_BF16 ? 2 : 4, g = Hq / Hkv;
   AttnArgs a = {};

@@ -1065,8 +1065,8 @@ def attention_fwd(plan: AttentionPlan, q: torch.Tensor, k: torch.Tensor, v: torc
     """coin_attention_fwd: q [B, Lq, Hq, D], k, v [B, Lk, Hkv, D] (`chunked_heads`) -> out [B, Lq, Hq, D] and, where a backward follows
     (`keep`), log2 of the rows' sums and (bfloat16) what rounding took from out."""
     b, lq, lk, hq, hkv, d = plan.dims
-    if not 0.0 < scale < 3.0e38:
-        raise CoinHipError(f"attention: scale must be positive and finite, got {scale}")
+    if not 0.0 < scale <= 1.0e30:
+        raise CoinHipError(f"attention: scale must be positive and at most 1e30, got {scale}")
     if key_lengths is not None and (key_lengths.dtype != torch.int32 or key_lengths.shape != (b,) or not key_lengths.is_contiguous()):
         raise CoinHipError(f"attention: key_lengths must be a contiguous int32 [{b}] tensor")
     index = _device_of(q, k, v, key_lengths)
@@ -1171,7 +1171,7 @@ def chunked_rows(x: torch.Tensor) -> torch.Tensor:
 def _pitch(x: Optional[torch.Tensor]) -> int:
     if x is None:
         return 0
-    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), (x.shape[1] + 7) // 8 * 8)
+    return x.stride(0) if x.shape[0] > 1 else (x.shape[1] + 7) // 8 * 8   # one row has no pitch of its own
 
 
 @functools.lru_cache(_WS_CACHE)

@@ -470,8 +470,8 @@ int coin_ema_update(const coin_ema_tensor* table, int num_tensors, int64_t max_n
  *   gives zeros and takes no gradient.
  * n_b = key_lengths[b] (device, clamped to 0 .. Lk) or Lk where key_lengths is NULL; k and v behind it are not used, whatever they hold.
  * *_strides: HOST arrays of three element strides (sequence, token, head); the last dimension is contiguous.  Pointers and strides are
- * multiples of 16 bytes (COIN_EALIGN), strides may be 0; 66 tokens' span below 2^31 bytes, D <= 128 and a multiple of 8 (bf16) / 4 (f32)
- * (COIN_ESHAPE); scale > 0.
+ * multiples of 16 bytes (COIN_EALIGN), strides may be 0; 130 tokens' span below 2^31 bytes, D <= 128 and a multiple of 8 (bf16) / 4 (f32)
+ * (COIN_ESHAPE); 0 < scale <= 1e30.
  * lse (float32 [B][Hkv][Lq * Hq / Hkv], or NULL when no backward follows): log2 of the row's sum of exp, +inf without a key.
  * out_lo (bfloat16, contiguous like out, 16-byte aligned, or NULL when no backward follows; not used in float32): what rounding took from out.
  * workspace: coin_attention_workspace_bytes (0: none), 16-byte aligned. */

@@ -447,6 +447,27 @@ def test_residual_norm_gradients_of_some_operands_alone():
             assert torch.equal(v, full[k]), (names, k)
 
 
+def test_linear_one_row_of_any_pitch():
+    base = rand((3, 77), BF16, 1)
+    w = rand((40, 72), BF16, 2, 0.1)
+    check_linear(base[1:2, 3:75], w, None, rand((1, 40), BF16, 3), "gelu", "one row, unaligned")
+    check_linear(base[:1, :72], w, None, rand((3, 45), BF16, 3)[2:, :40], "none", "one row of a pitch of 77")
+    v = rand((72,), BF16, 4).requires_grad_()                       # a vector
+    y = L.fused_linear(v, w, act=L.ACT_SILU, residual=rand((40,), BF16, 5))
+    g, = torch.autograd.grad(y, v, rand((40,), BF16, 6))
+    assert y.shape == (40,) and g.shape == (72,)
+
+
+def test_rms_norm_takes_its_default_epsilon_from_its_input():
+    m, q = torch.nn.RMSNorm(64, device=DEV), torch.nn.RMSNorm(64, device=DEV)
+    x, y = torch.zeros(3, 64, device=DEV), torch.full((3, 64), 2.0 ** -9, device=DEV, dtype=BF16)
+    r, h = L.residual_norm(x, y, post_norm=m, pre_norm=q)
+    # y's epsilon is bfloat16's 2^-7: y / sqrt(2^-18 + 2^-7); r's float32's
+    want = 2.0 ** -9 / (2.0 ** -18 + 2.0 ** -7) ** 0.5
+    within(r, torch.full_like(r, want).double(), torch.full_like(r, 2.0 ** -22).double(), "post")
+    within(h, torch.full_like(r, want / (want * want + 2.0 ** -23) ** 0.5).double(), torch.full_like(r, 2.0 ** -8).double(), "pre")
+
+
 def test_linear_master_weights_through_the_shadow():
     x, w, b = rand((70, 64), BF16, 1), rand((40, 64), F32, 2, 0.1), rand((40,), F32, 3)
     check_linear(x, w, b, None, "quick_gelu", "float32 master")
