@@ -587,20 +587,25 @@ struct Tiling {
   int ts, split;
 };
 
-// Tile size and K pieces of one product.  bfloat16: 256 x 256 tiles where their last round over the CUs is at least three quarters full on average;
-// else 128 x 128 where they fill the CUs, else 64 x 64; if even those are fewer than the CUs, the contraction is cut so that they become two
-// per CU, in pieces of at least four stages
+// Tile size and K pieces of one product; us measured with each size forced, 256 / 128 / 64:
+//   bfloat16: 256 x 256 tiles where at least 7 of 8 CUs work in every round.  [4096 x 4096 x 1024], one full round, 42 / 47 / 66; 192 tiles
+//     ([3000 x 4096]) 38 / 38 / 49; one and a half rounds ([6000 x 4096]) 72 / 66 / 92.  (float32 gains nothing: 304 / 280 / 302)
+//   128 x 128 where they are as many as the CUs: [2048 x 2048 x 2048] - / 30 / 32, float32 - / 139 / 146;
+//   fewer of them, with the contraction cut to two workgroups per CU, where the pieces keep 16 stages: [512 x 2048 x 8192] - / 38 / 83, float32
+//     - / 148 / 216; [2048 x 1024 x 8192] - / 49 / 56; shorter pieces pay for the join: [1024 x 2048 x 2048], 8 stages, - / 27 / 17;
+//   else 64 x 64; fewer than the CUs are cut the same way, in pieces of at least four stages
 static Tiling plan(int64_t M, int64_t N, int64_t K, int es) {
   const int64_t nk = (K * es + BKB - 1) / BKB;
-  const int64_t t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 127) / 128 * ((N + 127) / 128);
+  const int64_t t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 127) / 128 * ((N + 127) / 128), t64 = (M + 63) / 64 * ((N + 63) / 64);
   const int64_t rounds = (t256 + CUS - 1) / CUS;
-  if (es == 2 && 4 * t256 >= 3 * rounds * CUS) return {256, 1};
-  const int ts = t128 >= CUS ? 128 : 64;
-  const int64_t t = ts == 128 ? t128 : (M + 63) / 64 * ((N + 63) / 64);
-  int64_t s = t >= CUS ? 1 : 2 * CUS / t;
+  if (es == 2 && 8 * t256 >= 7 * rounds * CUS) return {256, 1};
+  if (t128 >= CUS) return {128, 1};
+  int64_t s = 2 * CUS / t128;
+  if (s <= 64 && nk / s >= 16) return {128, (int)s};
+  s = t64 >= CUS ? 1 : 2 * CUS / t64;
   if (s > nk / 4) s = nk / 4;
   if (s > 64) s = 64;
-  return {ts, s < 1 ? 1 : (int)s};
+  return {64, s < 1 ? 1 : (int)s};
 }
 
 static size_t part_bytes(int64_t M, int64_t N, int64_t K, int es) {

@@ -383,7 +383,7 @@ def check_linear(x, w, b, res, act, what):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 8, 8), (3, 77, 5), (4, 2048, 256), (16, 512, 520), (17, 40, 1000), (100, 1001, 33), (693, 512, 2048), (130, 136, 264),
-                                   (2000, 96, 96), (777, 64, 7), (2048, 1024, 2112), (5092, 384, 200), (3500, 264, 3601), (4000, 3400, 72)])
+                                   (2000, 96, 96), (777, 64, 7), (2048, 1024, 2112), (5092, 384, 200), (3500, 264, 3601), (4000, 3400, 72), (1000, 8200, 1100), (3840, 200, 3808)])
 def test_linear_sizes(m, k, n, dtype):
     i = (m + k + n) % 5
     act = list(ACTS)[i]
