@@ -39,6 +39,7 @@ struct AttnArgs {
   const int* lengths;                 // [B] or null
   int64_t qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];   // element strides: sequence, token, head
   int B, Lq, Lk, Hkv, g, D, R;
+  unsigned magic;                     // ceil(2^32 / g)
   int causal, splits, chunk;          // splits of the keys (forward; `chunk` keys each) or of the rows (dK, dV)
   float scale, c;                     // c = scale * log2 e
   float *part, *part_ml;
@@ -97,11 +98,18 @@ __device__ __forceinline__ int keys_of(const AttnArgs& p, int b) {
   return n < 0 ? 0 : (n > p.Lk ? p.Lk : n);
 }
 
+// t / g.  umulhi(t, magic) is the quotient or one more (the excess t (magic g - 2^32) / (g 2^32) is below 1 for 32-bit t)
+__device__ __forceinline__ int row_token(const AttnArgs& p, int t) {
+  if (p.g == 1) return t;
+  const int q = (int)__umulhi((unsigned)t, p.magic);
+  return q * p.g > t ? q - 1 : q;
+}
+
 // first key that row t does not see
 __device__ __forceinline__ int row_limit(const AttnArgs& p, int t, int n) {
   if (t >= p.R) return 0;
   if (!p.causal) return n;
-  const int i = p.g == 1 ? t : t / p.g;
+  const int i = row_token(p, t);
   const int l = i + n - p.Lq + 1;
   return l < 0 ? 0 : (l > n ? n : l);
 }
@@ -138,7 +146,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
   const int n = keys_of(p, b), nchunk = p.D / C::EL;
   const int t = (tile * NW + wave) * 32 + (lane & 31);
   const bool live = t < p.R;
-  const int i = p.g == 1 ? t : t / p.g, gi = t - i * p.g;
+  const int i = row_token(p, t), gi = t - i * p.g;
   const int lim = row_limit(p, t, n);
   const int wt = (tile * NW + wave) * 32, wlast = wt + 31 < p.R ? wt + 31 : p.R - 1;
   const int wmax = wt < p.R ? row_limit(p, wlast, n) : 0;                       // keys any row of the wave sees
@@ -306,7 +314,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
   }
   if (bad) l = lw = __builtin_nanf("");
   const float inv = lw == 0.f ? 0.f : 1.f / lw;
-  const int bh = (int)(row / p.R), t = (int)(row - (int64_t)bh * p.R), b = bh / p.Hkv, hk = bh - b * p.Hkv, i = t / p.g, gi = t - i * p.g;
+  const int bh = (int)(row / p.R), t = (int)(row - (int64_t)bh * p.R), b = bh / p.Hkv, hk = bh - b * p.Hkv, i = row_token(p, t), gi = t - i * p.g;
   if (p.lse && lane == 0) p.lse[row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
   if (d < p.D) {
     T* op = (T*)p.out + b * p.os[0] + (int64_t)i * p.os[1] + (int64_t)(hk * p.g + gi) * p.os[2] + d;
@@ -337,7 +345,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
   const int n = keys_of(p, b), nchunk = p.D / C::EL;
   const int t = (tile * NW + wave) * 32 + (lane & 31);
   const bool live = t < p.R;
-  const int i = p.g == 1 ? t : t / p.g, gi = t - i * p.g;
+  const int i = row_token(p, t), gi = t - i * p.g;
   const int lim = row_limit(p, t, n);
   const int wt = (tile * NW + wave) * 32, wlast = wt + 31 < p.R ? wt + 31 : p.R - 1;
   const int wmax = wt < p.R ? row_limit(p, wlast, n) : 0;
@@ -483,15 +491,15 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
   const unsigned gl = (unsigned)(p.dos[1] * sizeof(T)), gh = (unsigned)(p.dos[2] * sizeof(T));
   auto stage = [&](int tt, int buf) {
     char* d = lds + buf * 2 * TILE;
-    const int i0 = p.g == 1 ? tt : tt / p.g;
+    const int i0 = row_token(p, tt);
     stage_tile<ROWB, KT, NW, ROWB == 256>(d, qbase + (int64_t)i0 * p.qs[1], te - tt, nchunk, wave, lane, [&](int r) {
       if (p.g == 1) return (unsigned)r * ql;
-      const int x = tt + r, i = x / p.g;
+      const int x = tt + r, i = row_token(p, x);
       return (unsigned)(i - i0) * ql + (unsigned)(x - i * p.g) * qh;
     });
     stage_tile<ROWB, KT, NW, ROWB == 256>(d + TILE, gbase + (int64_t)i0 * p.dos[1], te - tt, nchunk, wave, lane, [&](int r) {
       if (p.g == 1) return (unsigned)r * gl;
-      const int x = tt + r, i = x / p.g;
+      const int x = tt + r, i = row_token(p, x);
       return (unsigned)(i - i0) * gl + (unsigned)(x - i * p.g) * gh;
     });
   };
@@ -760,7 +768,7 @@ extern "C" int coin_attention_fwd(const void* q, const int64_t* q_strides, const
   a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.lengths = key_lengths;
   set3(a.qs, q_strides); set3(a.os, out_strides);
   if (Lk > 0) { set3(a.ks, k_strides); set3(a.vs, v_strides); }
-  a.B = B; a.Lq = Lq; a.Lk = Lk; a.Hkv = Hkv; a.g = g; a.D = D; a.R = Lq * g;
+  a.B = B; a.Lq = Lq; a.Lk = Lk; a.Hkv = Hkv; a.g = g; a.D = D; a.R = Lq * g; a.magic = (unsigned)(((1ull << 32) + g - 1) / g);
   a.causal = causal != 0; a.splits = pl.fsplits; a.chunk = pl.fchunk; a.scale = scale; a.c = scale * LOG2E;
   a.part = (float*)workspace;
   a.part_ml = a.part + (size_t)pl.fsplits * B * Hkv * a.R * D;
@@ -798,7 +806,7 @@ extern "C" int coin_attention_bwd(const void* q, const int64_t* q_strides, const
   if (((uintptr_t)workspace | (uintptr_t)out_lo) & 15) return COIN_EALIGN;
   a.lo = (bf16_t*)const_cast<void*>(out_lo);
   a.q = q; a.k = k; a.v = v; a.o = out; a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.lse = const_cast<float*>(lse); a.lengths = key_lengths;
-  a.B = B; a.Lq = Lq; a.Lk = Lk; a.Hkv = Hkv; a.g = g; a.D = D; a.R = Lq * g;
+  a.B = B; a.Lq = Lq; a.Lk = Lk; a.Hkv = Hkv; a.g = g; a.D = D; a.R = Lq * g; a.magic = (unsigned)(((1ull << 32) + g - 1) / g);
   a.causal = causal != 0; a.splits = pl.ksplits; a.scale = scale; a.c = scale * LOG2E;
   a.delta = (float*)workspace;
   a.part = (float*)((char*)workspace + ((size_t)B * Hkv * a.R * sizeof(float) + 255) / 256 * 256);
