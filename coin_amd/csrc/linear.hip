@@ -272,7 +272,9 @@ __device__ __forceinline__ void put_tile(char* lds, const f32x16& acc, int row0,
   }
 }
 
-// C tile TS x TS by four waves (2 x 2), each (TS / 2)^2 in 32 x 32 accumulators, a ring of NST stages.  128 x 128 x 2 stages: 64 KiB of LDS,
+// C tile TS x TS by four waves (2 x 2), each (TS / 2)^2 in 32 x 32 accumulators, a ring of NST stages.  Bound by the DMA's traffic in bfloat16 (a
+// 128 x 128 tile moves twice the bytes a product of a 256 x 256 one: [2048 x 4096 x 1024] 25 us, 687 TFLOP/s), by the matrix instructions in float32
+// ([4096 x 4096 x 1024] 277 us, 124 TFLOP/s).  128 x 128 x 2 stages: 64 KiB of LDS,
 // two workgroups per CU, one's epilogue and barriers under the other's matrix instructions; 64 x 64 x 3: 48 KiB, three per CU
 template <typename T, bool AA, bool BA, int TS, int NST>
 __global__ __launch_bounds__(256, 2) void linear_gemm_kernel(const LinArgs p) {
@@ -343,6 +345,9 @@ __global__ __launch_bounds__(256, 2) void linear_gemm_kernel(const LinArgs p) {
 // 8 g + 6, and their K-tile g + 2 is issued in phases 3, 2, 4 of K-tile g and 1 of K-tile g + 1.  The order of issue is Bl Al Bh Ah, and each is
 // read by everybody in the phase after the wait that leaves the five youngest half-tiles (ten instructions of a wave) under way: fourteen
 // intervals to land.  K-tiles behind the last are issued too, out of range: they write zeros that nobody reads and keep the count.
+// [16381 x 2048 x 8192]: dx 530 us (1036 TFLOP/s), dW 507 us (1085), forward 510 us without an epilogue and 700 us with GELU, its slope and a
+// residual (0.8 GB of rows, 117 us of vector instructions, under nobody's matrix instructions).  Bound by LDS, which the DMA and the fragment
+// reads contend for: 340 us with every DMA out of range, 310 us without the reads.  128 x 128 tiles: 887 / 751 / 698 us (forward / dx / dW).
 // (bfloat16 alone: float32 matrix instructions are sixteen times slower, and 128 x 128 tiles already feed them)
 template <bool AA, bool BA>
 __global__ __launch_bounds__(512, 2) void linear_gemm256_kernel(const LinArgs p) {
@@ -469,7 +474,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const LinArgs p) {
   finish8<T>(p, v, bias, residual_ahead(p, row, col), row, col);
 }
 
-// dz = dy o act' (rows of ldz elements, zeros behind N) and the column sums of dz per block of rows.  32 threads x 8 columns, 8 rows at a time
+// dz = dy o act' (rows of ldz elements, zeros behind N) and the column sums of dz per block of rows.  32 threads x 8 columns, 8 rows at a time.
+// Bound by memory: [16381 x 8192] bfloat16 186 us at 4.3 TB/s
 struct DzArgs {
   const void* dy; int64_t ldy; int dy_f32;
   const void* slope; int64_t lds_;
@@ -569,7 +575,7 @@ __global__ __launch_bounds__(256) void linear_db_kernel(const float* part, void*
   else ((bf16_t*)db)[col] = (bf16_t)s;
 }
 
-// rows of `cols` elements -> rows of `ldd` elements, zeros behind the columns
+// rows of `cols` elements -> rows of `ldd` elements, zeros behind the columns (bound by memory; only rows that are not whole 16-byte chunks come here)
 template <typename T>
 __global__ __launch_bounds__(256) void pad_rows_kernel(const T* src, int64_t lds_, T* dst, int64_t ldd, int64_t rows, int cols) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, n8 = ldd / 8;
