@@ -13,7 +13,8 @@
 // accumulator is rescaled a few times per row instead of once per tile.
 //
 // D_i takes what rounding took from o_i back: bfloat16 training keeps that part beside o (`out_lo`).  Rows of few keys have o_i near a v_j, and
-// the rounded o_i alone made dQ and dK of a causal [77 x 77] head 10 % less exact.
+// the rounded o_i alone made dQ and dK of a causal [77 x 77] head 8 % less exact
+// (2-norm, 2.61e-3 against 2.41e-3).
 //
 // Backward, from L_i = log2 sum_j exp2(s_ij log2 e) that the forward keeps: P is recomputed, never stored.
 //   D_i = do_i . o_i,   dS = P (dO V^T - D),   dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO
@@ -127,8 +128,10 @@ struct Cfg {
 
 // ------------------------------------------------------------------------------------------------------------------------------ forward
 // 128 rows by four waves where that many workgroups fill the chip, else 32 rows by one; a wave's 32 rows keep Q (32 registers at D 128), the
-// scores of 64 keys (32) and O (64) within the 256 that let two waves on a SIMD (one wave: 256 us instead of 165 on the long case below).
-// Bound by issue: per 64 keys and 32 rows of D 128, 1024 cycles of matrix instructions beside about 1200 of exponentials, sums and conversions.
+// scores of 64 keys (32) and O (64) within the 256 that let two waves on a SIMD (workgroups of one wave, each with its
+// own tiles: 480 us instead of 199 on the long case below, one card).
+// Bound by issue: on that case the matrix units are busy 42 % of the SIMDs' cycles and vector instructions (exponentials, sums, conversions and the
+// issue of the products) 59 %.
 // 2 x 4001 causal tokens, 16 heads over 4, D 128, bfloat16: 181 us, 724 TFLOP/s.  One row per sequence over a long cache is bound by memory:
 // 16 ragged caches of up to 32768 keys, 278 us at 4.1 TB/s.
 template <typename T, int DP, int NW, bool SPLIT>
@@ -442,12 +445,12 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
 
 // -------------------------------------------------------------------------------------------------------------------- backward: dK and dV
 // A wave owns 32 keys and both accumulators (128 registers at D 128) and walks the rows; bound by the little room that leaves: 246 registers, two
-// waves a SIMD, 48 % of the matrix instructions' cycles.  2 x 4001 causal tokens as above: 380 us, 690 TFLOP/s over its four products.
+// waves a SIMD, matrix units busy 36 % of the cycles.  2 x 4001 causal tokens as above: 380 us, 690 TFLOP/s over its four products.
 template <typename T, int DP, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_dkv_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
-  // bfloat16, D 128: the fragments of K (32 registers), of V (32) and the two accumulators (128) leave too little of 256 registers (spilled:
-  // 690 us, 590 us with V in LDS); V's 32 KiB beside tiles of 32 rows still let two workgroups on a CU
+  // bfloat16, D 128: the fragments of K (32 registers), of V (32) and the two accumulators (128) leave too little of 256 registers (2 x 4001
+  // causal tokens: 401 us, 390 us with V in LDS and no spill, one card); V's 32 KiB beside tiles of 32 rows still let two workgroups on a CU
   constexpr bool VL = sizeof(T) == 2 && DP == 128 && NW == 4;
   constexpr int ROWB = C::ROWB, KT = VL ? 32 : C::KT, NS = KT / 32;
   using I = Img<ROWB, KT, ROWB == 256>;
@@ -636,7 +639,9 @@ constexpr int64_t SPAN = 0x7fffffff;
 
 static int cus() { return 256; }   // MI355X
 
-// Keys per split of the forward: workgroups of one wave (32 rows) would leave the chip idle when there are few rows
+// Keys per split of the forward: workgroups of one wave (32 rows) would leave the chip idle when there are few rows.  Measured on one token over 16
+// ragged caches of up to 32768 keys, 32 heads over 8: 4 workgroups a CU 294 + 6 us of joining, 8 289 + 11, 16 298 + 18; the lengths are ragged, so
+// the finer of the two that tie
 static int fwd_splits(int64_t wgs, int Lk, int* chunk) {
   *chunk = Lk;
   if (wgs <= 0 || wgs >= 2 * cus() || Lk <= 512) return 1;
@@ -653,7 +658,7 @@ static int fwd_waves(int64_t R, int64_t nbh) { return (R + 127) / 128 * nbh >= c
 
 // Row splits of the dK, dV launch: its workgroups (128 keys of a head) run two to a CU, and a causal head's are unequal, so two rounds' worth
 // are wanted while there are 512 rows for each.  Measured on 2 x 4001 causal tokens, 16 heads over 4, D 128 (256 workgroups unsplit): no split
-// 978 us, two splits 592 + 15 us of joining, four 406 + 25, eight 425 + 45
+// 976 us, two splits 563 + 15 us of joining, four 390 + 25, eight 410 + 45
 static int dkv_splits(int64_t wgs, int64_t R) {
   if (wgs <= 0) return 1;
   int64_t s = (4 * cus() + wgs - 1) / wgs;

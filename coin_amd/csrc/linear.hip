@@ -233,8 +233,8 @@ __device__ __forceinline__ void finish_rows(const LinArgs& p, const char* lds, i
   if (col >= p.N) return;
   float bias[8];
   if (p.split == 1) load_bias(p, bias, col);
-  // a rolled loop: the epilogue runs once a tile, and unrolled it is larger than the instruction cache (14 us a tile of 256 x 256).  The next
-  // row's residual is on its way while this one is finished
+  // a rolled loop: unrolled it takes the same time (789 and 790 us with GELU, its slope and a residual on [16381 x 2048 x 8192], one card) and
+  // 0.5 MB more code.  The next row's residual is on its way while this one is finished
   const int r0 = threadIdx.x / TPR;
   bf16x8 ahead = residual_ahead(p, mp + r0 < p.M ? mp + r0 : p.M - 1, col);
 #pragma unroll 1
@@ -273,8 +273,8 @@ __device__ __forceinline__ void put_tile(char* lds, const f32x16& acc, int row0,
 }
 
 // C tile TS x TS by four waves (2 x 2), each (TS / 2)^2 in 32 x 32 accumulators, a ring of NST stages.  Bound by the DMA's traffic in bfloat16 (a
-// 128 x 128 tile moves twice the bytes a product of a 256 x 256 one: [2048 x 4096 x 1024] 25 us, 687 TFLOP/s), by the matrix instructions in float32
-// ([4096 x 4096 x 1024] 277 us, 124 TFLOP/s).  128 x 128 x 2 stages: 64 KiB of LDS,
+// 128 x 128 tile moves twice the bytes a product of a 256 x 256 one: [2048 x 4096 x 1024] 25.3 us, 679 TFLOP/s), by the matrix instructions in float32
+// ([4096 x 4096 x 1024] 280 us, 123 TFLOP/s).  128 x 128 x 2 stages: 64 KiB of LDS,
 // two workgroups per CU, one's epilogue and barriers under the other's matrix instructions; 64 x 64 x 3: 48 KiB, three per CU
 template <typename T, bool AA, bool BA, int TS, int NST>
 __global__ __launch_bounds__(256, 2) void linear_gemm_kernel(const LinArgs p) {
@@ -346,8 +346,8 @@ __global__ __launch_bounds__(256, 2) void linear_gemm_kernel(const LinArgs p) {
 // read by everybody in the phase after the wait that leaves the five youngest half-tiles (ten instructions of a wave) under way: fourteen
 // intervals to land.  K-tiles behind the last are issued too, out of range: they write zeros that nobody reads and keep the count.
 // [16381 x 2048 x 8192]: dx 530 us (1036 TFLOP/s), dW 507 us (1085), forward 510 us without an epilogue and 700 us with GELU, its slope and a
-// residual (0.8 GB of rows, 117 us of vector instructions, under nobody's matrix instructions).  Bound by LDS, which the DMA and the fragment
-// reads contend for: 340 us with every DMA out of range, 310 us without the reads.  128 x 128 tiles: 887 / 751 / 698 us (forward / dx / dW).
+// residual (0.8 GB of rows that nobody's matrix instructions cover).  Bound by LDS, which the DMA and the fragment reads contend for: dx takes
+// 340 us with every DMA out of range, 500 us without the matrix instructions, 310 us with the DMA alone.  128 x 128 tiles: 887 / 751 / 698 us (forward / dx / dW).
 // (bfloat16 alone: float32 matrix instructions are sixteen times slower, and 128 x 128 tiles already feed them)
 template <bool AA, bool BA>
 __global__ __launch_bounds__(512, 2) void linear_gemm256_kernel(const LinArgs p) {
