@@ -474,9 +474,9 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
   const int n = keys_of(p, b), nchunk = p.D / C::EL;
   const int k0 = tile * NW * 32, kw = k0 + wave * 32, key = kw + (lane & 31);
   const bool live = key < n;
-  // rows that see a key of this tile: i >= k0 - n + Lq
+  // rows that see a key of this tile: i >= k0 - n + Lq (below Lq, so i g fits: a tile behind the sequence's length has no rows to start from)
   int t0 = 0;
-  if (p.causal) {
+  if (p.causal && k0 < n) {
     const int i0 = k0 - n + p.Lq;
     t0 = i0 > 0 ? i0 * p.g : 0;
   }

@@ -11,9 +11,9 @@
 // from x and y (not from the rounded r), so its normalised rows are exactly the forward's; only the rows' means and deviations (four
 // floats a row) are kept from the forward.  A row lives in the registers of TPR threads, two passes over registers give mean and variance.
 // 32768 rows of 2048, float32 stream, bfloat16 branch, gate and both norms: forward 156 us at 5.2 TB/s, backward 298 us at 4.05 TB/s (a copy of
-// 2 GiB: 4.8), its column sums 15 + 7 us.  All sums are float32.  The backward's `walkers` (TPR threads each) own contiguous rows and hold the column sums of dw, db and dgate in
-// registers; the walkers of a workgroup meet in LDS, the workgroups in a second launch that adds them in order: no atomics, the same
-// bits every time.
+// 2 GiB: 4.8), its column sums 15 + 7 us.  All sums are float32.  The backward's `walkers` (TPR threads each) own contiguous rows and hold
+// the column sums of dw, db and dgate in registers; the walkers of a workgroup meet in LDS, the workgroups in a second launch that adds them
+// in order: no atomics, the same bits every time.
 #include "common.h"
 
 namespace {

@@ -171,6 +171,25 @@ def test_attention_reads_nothing_behind_the_lengths(dtype):
     torch.testing.assert_close(L.attention(q, k, v, causal=True, key_lengths=long)[2], clean[0][2], rtol=0, atol=0)
 
 
+def test_attention_many_heads_over_a_long_and_nearly_empty_buffer():
+    # 256 heads times the tokens behind the sequence pass 2^31: those tiles of keys have no rows to start from
+    q, k, v = rand((1, 1, 256, 8), BF16, 1), rand((1, 64, 1, 8), BF16, 2), rand((1, 64, 1, 8), BF16, 3)
+    lk = (1 << 23) + 300
+    bufs = []
+    for t in (k, v):
+        buf = torch.full((1, lk, 1, 8), float("nan"), device=DEV, dtype=BF16)
+        buf[:, :64] = t
+        bufs.append(buf.requires_grad_())
+    qq = q.clone().requires_grad_()
+    out = L.attention(qq, *bufs, causal=True, key_lengths=torch.tensor([64], device=DEV))
+    dout = rand(out.shape, BF16, 4)
+    dq, dk, dv = torch.autograd.grad(out, [qq] + bufs, dout)
+    ref = attention_oracle(q, k, v, True, 8 ** -0.5, None, dout)
+    for name, t in (("out", out.detach()), ("dq", dq), ("dk", dk[:, :64]), ("dv", dv[:, :64])):
+        within(t, *ref[name], name)
+    assert not dk[:, 64:].any() and not dv[:, 64:].any()
+
+
 def test_attention_gradient_against_differences():
     q, k, v = (rand((1, 6, 2, 8), F32, s, 0.7) for s in (1, 2, 3))
     n = torch.tensor([5], device=DEV, dtype=torch.int32)
