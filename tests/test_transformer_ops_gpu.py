@@ -598,6 +598,74 @@ def test_a_block_captured_and_replayed():
             assert all(torch.equal(a, b) for a, b in zip(graphs[i][1], want)), (turn, i)
 
 
+# ------------------------------------------------------------------------------------------ tensors of more than 2^31 elements
+def test_attention_of_a_cache_past_32_bits():
+    lk, heads = 300000, 64                                # element 2^31 (byte 2^32) is token 262144
+    q = rand((1, 1, heads, 128), BF16, 1).requires_grad_()
+    g = torch.Generator(device=DEV).manual_seed(2)
+    k, v = (torch.randn((1, lk, heads, 128), generator=g, device=DEV, dtype=BF16) for _ in range(2))
+    k[:, 262144:] *= 1.5                                  # the largest scores lie behind it
+    k.requires_grad_()
+    v.requires_grad_()
+    out = L.attention(q, k, v, causal=True, scale=0.5)
+    dout = rand(out.shape, BF16, 3)
+    grads = torch.autograd.grad(out, [q, k, v], dout)
+    with torch.no_grad():
+        again = L.attention(q, k, v, causal=True, scale=0.5)
+    for h in (0, 31, 63):
+        at = lambda t: t.detach()[:, :, h:h + 1]  # noqa: E731
+        ref = attention_oracle(at(q), at(k), at(v), True, 0.5, None, at(dout))
+        assert float(ref["dv"][0][:, 262144:].abs().amax()) > 0.01    # what is compared is there
+        within(at(again), *ref["out"], f"out of head {h}, no gradient")
+        for name, t in zip(("out", "dq", "dk", "dv"), (out,) + grads):
+            within(at(t), *ref[name], f"{name} of head {h}")
+
+
+def test_residual_norm_of_rows_past_32_bits():
+    m, d, n = 1_100_000, 2048, 96                         # element 2^31 is in row 1048576
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, y = (torch.randn((m, d), generator=g, device=DEV, dtype=BF16) for _ in range(2))
+    dr, dh = (torch.randn((m, d), generator=g, device=DEV, dtype=BF16) for _ in range(2))
+    gate = rand((d,), BF16, 2)
+    post, pre = make_norm(True, d, 10), make_norm(True, d, 20)
+
+    def run(a, b, ga, gb):
+        a, b = a.detach().requires_grad_(), b.detach().requires_grad_()
+        r, h = L.residual_norm(a, b, post_norm=post, gate=gate, scale=0.5, pre_norm=pre)
+        return [t.detach() for t in (r, h) + torch.autograd.grad([r, h], [a, b], [ga, gb])]
+
+    whole = run(x, y, dr, dh)
+    for first in (0, 1048576 - n // 2, m - n):            # a row's arithmetic is its own
+        s = slice(first, first + n)
+        assert all(torch.equal(a[s], b) for a, b in zip(whole, run(x[s], y[s], dr[s], dh[s]))), first
+
+
+@pytest.mark.parametrize("k,n,act", [(8192, 64, "none"), (64, 8192, "gelu")])
+def test_linear_of_rows_past_32_bits(k, n, act):
+    m, t = 300000, 100                                    # x and dx, or y, its slope and dz, have 2.46e9 elements
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn((m, k), generator=g, device=DEV, dtype=BF16).requires_grad_()
+    w, b = rand((n, k), BF16, 2, k ** -0.5).requires_grad_(), rand((n,), BF16, 3).requires_grad_()
+    y = L.fused_linear(x, w, b, act=ACTS[act])
+    dy = torch.zeros_like(y)
+    dy[-t:] = rand((t, n), BF16, 4)                       # the last rows alone have a gradient
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+    assert not dx[:-t].any()
+    X, W, B, G = (z.detach().double() for z in (x[-t:], w, b, dy[-t:]))
+    z = (X @ W.t() + B).requires_grad_()
+    a = act64(z, act)
+    slope, = torch.autograd.grad(a.sum(), z)
+    z, a, u = z.detach(), a.detach(), U[BF16]
+    ez = (k + 8) * 2.0 ** -24 * (X.abs() @ W.abs().t() + B.abs())
+    within(y.detach()[-t:], a, u * a.abs() + 1.2 * ez + 2.0 ** -19 * a.abs() + 1e-30, "y")
+    dz = G * slope
+    ebz = G.abs() * (2.0 ** -11 * slope.abs() + 2.0 ** -20 + 1.1 * ez + 2.0 ** -25 if act != "none" else 0.0)
+    edz = ebz + u * (dz.abs() + ebz)
+    within(dx[-t:], dz @ W, u * (dz @ W).abs() + (edz + (n + 8) * 2.0 ** -24 * dz.abs()) @ W.abs() + 1e-30, "dx")
+    within(dw, dz.t() @ X, u * (dz.t() @ X).abs() + (edz + (t + 64) * 2.0 ** -24 * dz.abs()).t() @ X.abs() + 1e-30, "dw")
+    within(db, dz.sum(0), u * dz.sum(0).abs() + (ebz + (t + 8) * 2.0 ** -24 * dz.abs()).sum(0) + 1e-30, "db")
+
+
 def test_sequences_of_no_tokens_and_batches_of_none():
     q, k = torch.zeros(2, 0, 4, 64, device=DEV, requires_grad=True), torch.zeros(2, 5, 4, 64, device=DEV, requires_grad=True)
     out = L.attention(q, k, k)
