@@ -47,9 +47,9 @@ struct AttnArgs {
 };
 
 // acc[dt]^T[d][col] += sum over the 32 image rows row0 .. row0 + 31 of image[row][d] * p[row][col], p in accumulator registers:
-// register r of lane half h holds row 8 (r >> 2) + 4 h + (r & 3)
-template <typename T, typename I, int ND>
-__device__ __forceinline__ void mma_t(f32x16 (&acc)[ND], const char* img, int row0, const f32x16& p, int lane) {
+// register r of lane half h holds row 8 (r >> 2) + 4 h + (r & 3).  SUM (bfloat16): sum[.][col] += the same with an image of ones
+template <typename T, typename I, int ND, bool SUM = false>
+__device__ __forceinline__ void mma_t(f32x16 (&acc)[ND], const char* img, int row0, const f32x16& p, int lane, f32x16* sum = nullptr) {
   const int half = lane >> 5;
   if constexpr (sizeof(T) == 2) {
     const int q4 = (lane >> 2) & 3, p4 = lane & 3, lrow = half * 4 + q4;
@@ -58,6 +58,10 @@ __device__ __forceinline__ void mma_t(f32x16 (&acc)[ND], const char* img, int ro
       bf16x8 pf;
 #pragma unroll
       for (int e = 0; e < 8; ++e) pf[e] = (bf16_t)p[8 * s + e];
+      if constexpr (SUM) {
+        const s16x8 one = {0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80};
+        *sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, one), pf, *sum, 0, 0, 0);
+      }
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) {
         const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + (p4 >> 1);
@@ -127,9 +131,8 @@ struct Cfg {
 };
 
 // ------------------------------------------------------------------------------------------------------------------------------ forward
-// 128 rows by four waves where that many workgroups fill the chip, else 32 rows by one; a wave's 32 rows keep Q (32 registers at D 128), the
-// scores of 64 keys (32) and O (64) within the 256 that let two waves on a SIMD (workgroups of one wave, each with its
-// own tiles: 480 us instead of 199 on the long case below, one card).
+// 128 rows by four waves, or up to 32 rows by one; a wave's 32 rows keep Q (32 registers at D 128), the scores of 64 keys (32) and O (64) within
+// the 256 that let two waves on a SIMD (workgroups of one wave, each with its own tiles: 480 us instead of 199 on the long case below, one card).
 // Bound by issue: on that case the matrix units are busy 42 % of the SIMDs' cycles and vector instructions (exponentials, sums, conversions and the
 // issue of the products) 59 %.
 // 2 x 4001 causal tokens, 16 heads over 4, D 128, bfloat16: 181 us, 724 TFLOP/s.  One row per sequence over a long cache is bound by memory:
@@ -177,9 +180,11 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
   f32x16 o[C::ND];
 #pragma unroll
   for (int d = 0; d < C::ND; ++d) o[d] = zero16();
-  // l: the sum that L is made of.  lw: the sum of the rounded probabilities that the product takes; o = sum p~ v / sum p~ is off by the
-  // roundings times (v_j - o) instead of v_j, which is what D and through it dQ and dK see
-  float m = -INFINITY, l = 0.f, lw = 0.f;
+  // l: the sum that L is made of.  lw[0]: the sum of the rounded probabilities that the product takes; o = sum p~ v / sum p~ is off by the
+  // roundings times (v_j - o) instead of v_j, which is what D and through it dQ and dK see.  It comes from the matrix units, as one more row
+  // of V^T that holds ones: the vector unit is the busier one (198 -> 191 us on the long case, one card)
+  float m = -INFINITY, l = 0.f;
+  f32x16 lw = zero16();
   const float c = p.c;
   if (kb < ke) stage(kb, 0);
   int buf = 0;
@@ -214,38 +219,32 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
       const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
       m = mn;
       l *= al;
-      lw *= al;
+      lw[0] *= al;
 #pragma unroll
       for (int d = 0; d < C::ND; ++d) o[d] *= al;
     }
     const float mc = m == -INFINITY ? 0.f : m * c;
-    float ls = 0.f, lr = 0.f;
+    float ls = 0.f;
 #pragma unroll
     for (int s = 0; s < C::NS; ++s)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         st[s][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[s][r], c, -mc));
         ls += st[s][r];
-        if constexpr (sizeof(T) == 2) {
-          st[s][r] = (float)(bf16_t)st[s][r];
-          lr += st[s][r];
-        }
       }
     l += ls;
-    if (sizeof(T) == 2) lw += lr;
 #pragma unroll
     for (int s = 0; s < C::NS; ++s)
-      if (sizeof(T) == 2 || kt + s * 32 < wmax) mma_t<T, I, C::ND>(o, vimg, s * 32, st[s], lane);
+      if (sizeof(T) == 2 || kt + s * 32 < wmax) mma_t<T, I, C::ND, sizeof(T) == 2>(o, vimg, s * 32, st[s], lane, &lw);
   }
   l += __shfl_xor(l, 32, 64);
-  lw += __shfl_xor(lw, 32, 64);
-  if (sizeof(T) == 4) lw = l;
+  const float lsum = sizeof(T) == 4 ? l : lw[0];
   if (!live) return;
   const size_t row = (size_t)bh * p.R + t;
   if (SPLIT) {   // unnormalised sums with their maximum; joined by attention_join_kernel.  A split without keys leaves l = 0 and no sums
     const size_t prow = (size_t)split * nbh * p.R + row;
     if (half == 0) {
-      *reinterpret_cast<f32x4*>(p.part_ml + prow * 4) = (f32x4){m == -INFINITY ? 0.f : m * c, l, lw, 0.f};
+      *reinterpret_cast<f32x4*>(p.part_ml + prow * 4) = (f32x4){m == -INFINITY ? 0.f : m * c, l, lsum, 0.f};
     }
     if (kb < wmax && l > 0.f) {
 #pragma unroll
@@ -258,7 +257,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
     }
     return;
   }
-  const float inv = lw > 0.f ? 1.f / lw : (lw == 0.f ? 0.f : lw);   // no key: zeros; NaN stays
+  const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);   // no key: zeros; NaN stays
   if (p.lse && half == 0) p.lse[row] = l == 0.f ? INFINITY : m * c + __builtin_amdgcn_logf(l);
   T* op = (T*)p.out + b * p.os[0] + (int64_t)i * p.os[1] + (int64_t)(hk * p.g + gi) * p.os[2];
   bf16_t* lp = p.lo ? p.lo + (((size_t)b * p.Lq + i) * p.Hkv * p.g + hk * p.g + gi) * p.D : nullptr;
@@ -340,9 +339,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
 
 // ----------------------------------------------------------------------------------------------------------------------- backward: dQ, D
 // The forward's split and tiles with dO beside Q; 2 x 4001 causal tokens as above: 212 us, 929 TFLOP/s over its three products.
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_dq_kernel(const AttnArgs p) {
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_dq_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
+  constexpr int NW = 4;
   using I = typename C::I;
   constexpr int ROWB = C::ROWB, KT = C::KT;
   __shared__ __attribute__((aligned(1024))) char lds[4 * C::TILE];
@@ -446,12 +446,15 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
 // -------------------------------------------------------------------------------------------------------------------- backward: dK and dV
 // A wave owns 32 keys and both accumulators (128 registers at D 128) and walks the rows; bound by the little room that leaves: 246 registers, two
 // waves a SIMD, matrix units busy 36 % of the cycles.  2 x 4001 causal tokens as above: 380 us, 690 TFLOP/s over its four products.
-template <typename T, int DP, int NW, bool SPLIT>
-__global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_dkv_kernel(const AttnArgs p) {
+template <typename T, int DP, bool SPLIT>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_dkv_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
-  // bfloat16, D 128: the fragments of K (32 registers), of V (32) and the two accumulators (128) leave too little of 256 registers (2 x 4001
-  // causal tokens: 401 us, 390 us with V in LDS and no spill, one card); V's 32 KiB beside tiles of 32 rows still let two workgroups on a CU
-  constexpr bool VL = sizeof(T) == 2 && DP == 128 && NW == 4;
+  constexpr int NW = 4;
+  // D 128: the fragments of K (32 registers in bfloat16, 64 in float32), of V (as many) and the two accumulators (128) leave too little of 256 or
+  // 512 registers.  With V in LDS and no spill: 2 x 4001 causal tokens, bfloat16, 401 -> 390 us (one card; V's 32 KiB beside tiles of 32 rows still
+  // let two workgroups on a CU); 4000 causal tokens, 32 heads over 8, float32, 2919 -> 2478 us.  Four waves at any size: workgroups of one wave took
+  // 347 us instead of 133 ([2 x 2001], 16 heads over 4, D 128, causal, bfloat16), and as long where there are few tokens
+  constexpr bool VL = DP == 128;
   constexpr int ROWB = C::ROWB, KT = VL ? 32 : C::KT, NS = KT / 32;
   using I = Img<ROWB, KT, ROWB == 256>;
   using IV = Img<ROWB, NW * 32, ROWB == 256>;
@@ -639,13 +642,16 @@ constexpr int64_t SPAN = 0x7fffffff;
 
 static int cus() { return 256; }   // MI355X
 
-// Keys per split of the forward: workgroups of one wave (32 rows) would leave the chip idle when there are few rows.  Measured on one token over 16
-// ragged caches of up to 32768 keys, 32 heads over 8: 4 workgroups a CU 294 + 6 us of joining, 8 289 + 11, 16 298 + 18; the lengths are ragged, so
-// the finer of the two that tie
-static int fwd_splits(int64_t wgs, int Lk, int* chunk) {
+// Keys per split of the forward.  Up to 32 rows (a few tokens over a cache): one wave a workgroup, 8 workgroups a CU where fewer than 2 a CU
+// would run.  Measured on one token over 16 ragged caches of up to 32768 keys, 32 heads over 8: 4 workgroups a CU 294 + 6 us of joining, 8
+// 289 + 11, 16 298 + 18; the lengths are ragged, so the finer of the two that tie.  More rows: four waves, 4 workgroups a CU where fewer than
+// one would run.  [1 x 16000] tokens, one head of 128, bfloat16: 277 us with one-wave workgroups in 5 splits, 123 with four waves in 9;
+// [1 x 500] over 20000 keys, 8 heads of 64: 74, 55; float32 [1 x 2048], 8 heads over 2 of 64: 152 unsplit, 99.  Pieces under 256 keys would pay
+// more for the join than they gain
+static int fwd_splits(int64_t wgs, int waves, int Lk, int* chunk) {
   *chunk = Lk;
-  if (wgs <= 0 || wgs >= 2 * cus() || Lk <= 512) return 1;
-  int64_t s = (8 * cus() + wgs - 1) / wgs, most = (Lk + 255) / 256;
+  if (wgs <= 0 || wgs >= (waves == 4 ? 1 : 2) * cus() || Lk <= 512) return 1;
+  int64_t s = ((waves == 4 ? 4 : 8) * cus() + wgs - 1) / wgs, most = (Lk + 255) / 256;
   if (s > most) s = most;
   if (s <= 1) return 1;
   int c = (int)((Lk + s - 1) / s);
@@ -654,34 +660,32 @@ static int fwd_splits(int64_t wgs, int Lk, int* chunk) {
   return (Lk + c - 1) / c;
 }
 
-static int fwd_waves(int64_t R, int64_t nbh) { return (R + 127) / 128 * nbh >= cus() ? 4 : 1; }
-
-// Row splits of the dK, dV launch: its workgroups (128 keys of a head) run two to a CU, and a causal head's are unequal, so two rounds' worth
-// are wanted while there are 512 rows for each.  Measured on 2 x 4001 causal tokens, 16 heads over 4, D 128 (256 workgroups unsplit): no split
-// 976 us, two splits 563 + 15 us of joining, four 390 + 25, eight 410 + 45
+// Row splits of the dK, dV launch: its workgroups (128 keys of a head) run two to a CU (D 128 float32: one), and a causal head's are unequal, so
+// two rounds' worth are wanted while there are 512 rows for each; where half the chip would idle, one round's worth down to 128 rows each.
+// 2 x 4001 causal tokens, 16 heads over 4, D 128 (256 workgroups unsplit): no split 976 us, two 563 + 15 us of joining, four 390 + 25, eight
+// 410 + 45.  [1 x 1000], 8 heads of 64 (64 workgroups): unsplit 42 us, 7 splits 23 with the join; [4 x 333], 16 heads of 128 (192): unsplit 29, two 36
 static int dkv_splits(int64_t wgs, int64_t R) {
   if (wgs <= 0) return 1;
-  int64_t s = (4 * cus() + wgs - 1) / wgs;
+  int64_t s = (4 * cus() + wgs - 1) / wgs, fill = 2 * wgs <= cus() ? 2 * cus() / wgs : 1;
   if (s > R / 512) s = R / 512;
+  if (fill > R / 128) fill = R / 128;
+  if (s < fill) s = fill;
   return s < 1 ? 1 : (int)s;
 }
 
-static int dkv_waves(int64_t Lk, int64_t nbh) { return (Lk + 127) / 128 * nbh >= cus() ? 4 : 1; }
-
 struct Plan {
-  int fw, fsplits, fchunk, kw, ksplits;
+  int fw, fsplits, fchunk, ksplits;
   size_t fwd_bytes, bwd_bytes;
 };
 
 static Plan make_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D) {
   Plan p;
   const int64_t nbh = B * Hkv, R = Lq * (Hq / Hkv);
-  p.fw = fwd_waves(R, nbh);
-  p.fsplits = p.fw == 1 ? fwd_splits((R + 31) / 32 * nbh, (int)Lk, &p.fchunk) : 1;
-  if (p.fsplits == 1) p.fchunk = (int)Lk;
+  p.fw = R > 32 ? 4 : 1;
+  p.fsplits = fwd_splits((R + p.fw * 32 - 1) / (p.fw * 32) * nbh, p.fw, (int)Lk, &p.fchunk);
+  if (p.fsplits == 1) p.fw = 4;   // four waves stage a tile together, however few of them have rows ([4 x 333], 16 heads of 128: 32 us, 18)
   p.fwd_bytes = p.fsplits > 1 ? (size_t)p.fsplits * nbh * R * (D + 4) * sizeof(float) : 0;
-  p.kw = dkv_waves(Lk, nbh);
-  p.ksplits = dkv_splits((Lk + p.kw * 32 - 1) / (p.kw * 32) * nbh, R);
+  p.ksplits = dkv_splits((Lk + 127) / 128 * nbh, R);
   p.bwd_bytes = (size_t)nbh * R * sizeof(float);
   p.bwd_bytes = (p.bwd_bytes + 255) / 256 * 256;
   if (p.ksplits > 1) p.bwd_bytes += (size_t)p.ksplits * nbh * Lk * 2 * D * sizeof(float);
@@ -713,10 +717,9 @@ static void launch_fwd(const AttnArgs& a, const Plan& pl, hipStream_t st) {
   const int64_t nbh = (int64_t)a.B * a.Hkv;
   const unsigned grid = (unsigned)((a.R + pl.fw * 32 - 1) / (pl.fw * 32) * nbh * pl.fsplits);
   if (pl.fsplits > 1) {
-    attention_fwd_kernel<T, DP, 1, true><<<grid, 64, 0, st>>>(a);
+    if (pl.fw == 1) attention_fwd_kernel<T, DP, 1, true><<<grid, 64, 0, st>>>(a);
+    else attention_fwd_kernel<T, DP, 4, true><<<grid, 256, 0, st>>>(a);
     attention_join_kernel<T><<<(unsigned)((nbh * a.R + 3) / 4), 256, 0, st>>>(a);
-  } else if (pl.fw == 1) {
-    attention_fwd_kernel<T, DP, 1, false><<<grid, 64, 0, st>>>(a);
   } else {
     attention_fwd_kernel<T, DP, 4, false><<<grid, 256, 0, st>>>(a);
   }
@@ -726,20 +729,15 @@ template <typename T, int DP>
 static void launch_bwd(const AttnArgs& a, const Plan& pl, hipStream_t st) {
   const int64_t nbh = (int64_t)a.B * a.Hkv;
   if (a.R > 0) {
-    const unsigned grid = (unsigned)((a.R + pl.fw * 32 - 1) / (pl.fw * 32) * nbh);
-    if (pl.fw == 1) attention_dq_kernel<T, DP, 1><<<grid, 64, 0, st>>>(a);
-    else attention_dq_kernel<T, DP, 4><<<grid, 256, 0, st>>>(a);
+    attention_dq_kernel<T, DP><<<(unsigned)((a.R + 127) / 128 * nbh), 256, 0, st>>>(a);
   }
   if (a.Lk > 0) {
-    const unsigned grid = (unsigned)((a.Lk + pl.kw * 32 - 1) / (pl.kw * 32) * nbh * pl.ksplits);
+    const unsigned grid = (unsigned)((a.Lk + 127) / 128 * nbh * pl.ksplits);
     if (pl.ksplits > 1) {
-      if (pl.kw == 1) attention_dkv_kernel<T, DP, 1, true><<<grid, 64, 0, st>>>(a);
-      else attention_dkv_kernel<T, DP, 4, true><<<grid, 256, 0, st>>>(a);
+      attention_dkv_kernel<T, DP, true><<<grid, 256, 0, st>>>(a);
       attention_dkv_join_kernel<T><<<(unsigned)((nbh * a.Lk * 2 * a.D / 4 + 255) / 256), 256, 0, st>>>(a);
-    } else if (pl.kw == 1) {
-      attention_dkv_kernel<T, DP, 1, false><<<grid, 64, 0, st>>>(a);
     } else {
-      attention_dkv_kernel<T, DP, 4, false><<<grid, 256, 0, st>>>(a);
+      attention_dkv_kernel<T, DP, false><<<grid, 256, 0, st>>>(a);
     }
   }
 }

@@ -117,6 +117,25 @@ def test_attention_matches_its_definition(shape, dtype):
     check_attention(q, k, v, causal, n, str(shape))
 
 
+SPLIT_SHAPES = [   # keys (forward) and rows (dK, dV) in pieces, some of them empty
+    (2, 40, 1500, 4, 2, 64, True, [1500, 70]),
+    (1, 200, 1030, 4, 4, 128, False, [300]),
+    (1, 33, 2100, 2, 1, 32, True, [0]),
+    (1, 700, 700, 4, 2, 128, True, None),
+    (3, 1000, 129, 2, 1, 64, True, [129, 128, 1]),
+    (1, 32, 513, 2, 2, 128, True, None),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", SPLIT_SHAPES)
+def test_attention_in_pieces(shape, dtype):
+    b, lq, lk, hq, hkv, d, causal, lengths = shape
+    q, k, v = rand((b, lq, hq, d), dtype, 1), rand((b, lk, hkv, d), dtype, 2), rand((b, lk, hkv, d), dtype, 3)
+    n = torch.tensor(lengths, device=DEV, dtype=torch.int32) if lengths else None
+    check_attention(q, k, v, causal, n, str(shape))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_head_dimensions(dtype):
     for d in range(8, 129, 8) if dtype == BF16 else (4, 12, 32, 36, 64, 68, 100, 128):
