@@ -998,10 +998,15 @@ class _ResidualNorm(Function):
         nx, ny, ngate, npw, npb, nnw, nnb, _ = ctx.needs_input_grad
         # without a gate, a norm behind the branch or a scale, the branch's gradient IS the stream's
         same = y is not None and gate is None and post_eps is None and scale == 1.0 and y.dtype == x.dtype
+        through = dh is None   # r alone has a gradient: it is the stream's, as it stands
+        if through and (same or not (ny or ngate or npw or npb)):
+            return (dr if nx else None, dr if ny else None) + (None,) * 6
         dx, dy, dgate, dpw, dpb, dnw, dnb = K.residual_norm_bwd(
             x, y, gate, rows_per_gate, (pw, pb, post_eps) if post_eps is not None else None, (nw, None, pre_eps) if pre_eps is not None else None, rms, scale,
             stats, dr.contiguous() if dr is not None else None, dh.contiguous() if dh is not None else None, branch_dtype,
-            (nx or (same and ny), ny and not same, ngate, npw, npb, nnw and dh is not None, nnb and dh is not None))
+            ((nx or (same and ny)) and not through, ny and not same, ngate, npw, npb, nnw and not through, nnb and not through))
+        if through:
+            dx = dr
         return (dx if nx else None, (dx if ny else None) if same else dy, dgate, dpw, dpb, dnw, dnb, None)
 
 

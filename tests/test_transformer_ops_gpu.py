@@ -485,6 +485,35 @@ def test_residual_norm_gradients_of_some_operands_alone():
             assert torch.equal(v, full[k]), (names, k)
 
 
+def test_residual_norm_gradient_of_the_stream_alone():
+    x, y = (rand((3, 40, 96), F32, i).requires_grad_() for i in (1, 2))
+    gate = rand((3, 1, 96), F32, 3).requires_grad_()
+    ln, post = make_norm(False, 96, 10), make_norm(False, 96, 20)
+    dr = rand(x.shape, F32, 4)
+    for turn in range(2):                                 # r keeps a gradient of its own; nothing is written into the caller's
+        keep = dr.clone()
+        gx, gy = torch.autograd.grad(L.residual_norm(x, y, pre_norm=ln)[0], [x, y], dr)
+        assert torch.equal(gx, keep) and torch.equal(gy, keep) and torch.equal(dr, keep)
+    gx, gy, gg, gw = torch.autograd.grad(L.residual_norm(x, y, post_norm=post, gate=gate, scale=0.5, pre_norm=ln)[0], [x, y, gate, post.weight], dr)
+    X, Y, G, W, B = (t.detach().double().requires_grad_() for t in (x, y, gate, post.weight, post.bias))
+    want = torch.autograd.grad(X + 0.5 * G * torch.nn.functional.layer_norm(Y, (96,), W, B, 1e-5), [X, Y, G, W], dr.double())
+    assert torch.equal(gx, dr)
+    for name, a, b in zip(("dy", "dgate", "dw"), (gy, gg, gw), want[1:]):
+        # float32 sums of up to 120 products a value, relative to the largest
+        within(a, b, 256 * 2.0 ** -24 * b.abs().amax() + 0 * b, name)
+    g, = torch.autograd.grad(L.residual_norm(x, y.detach(), gate=gate.detach())[0].sum(), x)
+    assert torch.equal(g, torch.ones_like(x))
+    x.grad = y.grad = None
+    a, b = x * 2, y * 2                                   # leaves behind other operations, accumulated in place
+    L.residual_norm(a, b)[0].backward(dr)
+    L.residual_norm(x * 2, y * 2)[0].backward(dr)
+    assert torch.equal(x.grad, 4 * dr) and torch.equal(y.grad, 4 * dr)
+    x.grad = y.grad = None
+    for _ in range(2):                                    # the same gradient tensor for both leaves: neither accumulates into the other
+        L.residual_norm(x, y)[0].backward(dr)
+    assert torch.equal(x.grad, 2 * dr) and torch.equal(y.grad, 2 * dr) and torch.equal(dr, keep)
+
+
 def test_linear_one_row_of_any_pitch():
     base = rand((3, 77), BF16, 1)
     w = rand((40, 72), BF16, 2, 0.1)
