@@ -133,10 +133,10 @@ struct Cfg {
 // ------------------------------------------------------------------------------------------------------------------------------ forward
 // 128 rows by four waves, or up to 32 rows by one; a wave's 32 rows keep Q (32 registers at D 128), the scores of 64 keys (32) and O (64) within
 // the 256 that let two waves on a SIMD (workgroups of one wave, each with its own tiles: 480 us instead of 199 on the long case below, one card).
-// Bound by issue: on that case the matrix units are busy 42 % of the SIMDs' cycles and vector instructions (exponentials, sums, conversions and the
-// issue of the products) 59 %.
-// 2 x 4001 causal tokens, 16 heads over 4, D 128, bfloat16: 181 us, 724 TFLOP/s.  One row per sequence over a long cache is bound by memory:
-// 16 ragged caches of up to 32768 keys, 278 us at 4.1 TB/s.
+// Bound by issue: on that case the matrix units are busy 49 % of the SIMDs' cycles and vector instructions (exponentials, sums, conversions and the
+// issue of the products) 47 %, with two waves to cover one another.
+// 2 x 4001 causal tokens, 16 heads over 4, D 128, bfloat16: 179 us, 732 TFLOP/s.  One row per sequence over a long cache is bound by memory:
+// 16 ragged caches of up to 32768 keys, 276 us at 4.1 TB/s.
 template <typename T, int DP, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_fwd_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
@@ -338,7 +338,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
 }
 
 // ----------------------------------------------------------------------------------------------------------------------- backward: dQ, D
-// The forward's split and tiles with dO beside Q; 2 x 4001 causal tokens as above: 212 us, 929 TFLOP/s over its three products.
+// The forward's split and tiles with dO beside Q; 2 x 4001 causal tokens as above: 216 us, 912 TFLOP/s over its three products,
+// matrix units busy 57 % of the cycles.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_dq_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void at
 
 // -------------------------------------------------------------------------------------------------------------------- backward: dK and dV
 // A wave owns 32 keys and both accumulators (128 registers at D 128) and walks the rows; bound by the little room that leaves: 246 registers, two
-// waves a SIMD, matrix units busy 36 % of the cycles.  2 x 4001 causal tokens as above: 380 us, 690 TFLOP/s over its four products.
+// waves a SIMD, matrix units busy 39 % of the cycles.  2 x 4001 causal tokens as above: 358 us, 732 TFLOP/s over its four products.
 template <typename T, int DP, bool SPLIT>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void attention_dkv_kernel(const AttnArgs p) {
   using C = Cfg<T, DP>;
