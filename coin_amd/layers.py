@@ -1010,13 +1010,14 @@ class _ResidualNorm(Function):
         return (dx if nx else None, (dx if ny else None) if same else dy, dgate, dpw, dpb, dnw, dnb, None)
 
 
-def _norm_of(norm: Optional[torch.nn.Module], d: int, dtype: torch.dtype):
+def _norm_of(norm: Optional[torch.nn.Module], d: int):
     """(weight, bias, eps, is it an RMSNorm) of an nn.LayerNorm / nn.RMSNorm over rows of d."""
     if not isinstance(norm, (torch.nn.LayerNorm, torch.nn.RMSNorm)) or tuple(norm.normalized_shape) != (d,):
         raise CoinHipError(f"residual_norm: nn.LayerNorm({d}) or nn.RMSNorm({d}) expected, got {norm}")
     rms = isinstance(norm, torch.nn.RMSNorm)
     f32 = lambda p: None if p is None else (p if p.dtype == torch.float32 else p.float()).contiguous()  # noqa: E731
-    eps = norm.eps if norm.eps is not None else torch.finfo(dtype).eps
+    # an RMSNorm without an epsilon: the module computes bfloat16 rows in float32 too and takes that type's
+    eps = norm.eps if norm.eps is not None else torch.finfo(torch.float32).eps
     return f32(norm.weight), f32(getattr(norm, "bias", None)), float(eps), rms
 
 
@@ -1051,10 +1052,10 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_nor
     pw = pb = nw = nb = post_eps = pre_eps = None
     kinds = set()
     if post_norm is not None:
-        pw, pb, post_eps, rms = _norm_of(post_norm, d, y.dtype)
+        pw, pb, post_eps, rms = _norm_of(post_norm, d)
         kinds.add(rms)
     if pre_norm is not None:
-        nw, nb, pre_eps, rms = _norm_of(pre_norm, d, x.dtype)
+        nw, nb, pre_eps, rms = _norm_of(pre_norm, d)
         kinds.add(rms)
     if len(kinds) > 1:
         raise CoinHipError("residual_norm: both norms are LayerNorms or both are RMSNorms")

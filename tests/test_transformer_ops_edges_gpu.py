@@ -1,0 +1,45 @@
+"""Attention, residual norms and linear epilogues (coin_amd.layers) where a call meets the module, the layout or the mode that it stands for:
+default epsilons, wide pitches, column sums, rows that the mask leaves empty, infinities and NaN, forward-mode derivatives."""
+import pytest
+import torch
+
+from coin_amd import layers as L
+from test_transformer_ops_gpu import BF16, DEV, F32, U, rand, within
+
+pytestmark = pytest.mark.gpu
+
+
+# --------------------------------------------------------------------------------------------------------------- default epsilon
+@pytest.mark.parametrize("weight", [F32, BF16, None])
+@pytest.mark.parametrize("ts,tb", [(F32, F32), (F32, BF16), (BF16, BF16)])
+def test_rms_norm_without_an_epsilon_is_the_module(ts, tb, weight):
+    """Rows of 2^-10, whose mean square 2^-20 lies between the epsilons of float32 (2^-23) and bfloat16 (2^-7): on both sides, against the
+    modules that the call stands for and against the formula in 64 bits."""
+    d = 64
+    post, pre = (torch.nn.RMSNorm(d, elementwise_affine=weight is not None, device=DEV, dtype=weight or F32) for _ in range(2))
+    x, y = (rand((5, d), F32, 1) * 2.0 ** -10).to(ts), (rand((5, d), F32, 2) * 2.0 ** -10).to(tb)
+    _, h = L.residual_norm(x, pre_norm=pre, branch_dtype=tb)
+    r, _ = L.residual_norm(torch.zeros_like(x), y, post_norm=post)
+    norm64 = lambda t: t.double() / (t.double().pow(2).mean(-1, keepdim=True) + 2.0 ** -23).sqrt()  # noqa: E731
+    for got, src, module in ((h, x, pre), (r, y, post)):
+        want = norm64(src)
+        # a sum of 64 squares, a root and a quotient in float32: 80 steps of 2^-24 at most; then one rounding to the result's type
+        tol = (80 * 2.0 ** -24 + U[got.dtype]) * want.abs()
+        within(got, want, tol, "formula")
+        m = module(src)
+        within(got, m.double(), 2 * tol + (U[m.dtype] + 80 * 2.0 ** -24) * want.abs(), "module")
+
+
+def test_gradient_of_an_rms_norm_without_an_epsilon():
+    m = torch.nn.RMSNorm(96, device=DEV)
+    x = (rand((7, 96), F32, 1) * 2.0 ** -10).to(BF16).requires_grad_()
+    dh = rand((7, 96), BF16, 2)
+    gx, gw = torch.autograd.grad(L.residual_norm(x, pre_norm=m)[1], [x, m.weight], dh)
+    X, W = x.detach().double().requires_grad_(), torch.ones(96, device=DEV, dtype=torch.float64, requires_grad=True)
+    rstd = (X.pow(2).mean(-1, keepdim=True) + 2.0 ** -23).rsqrt()
+    want = torch.autograd.grad(X * rstd * W, [X, W], dh.double())
+    # float32 sums of 96 products: 128 steps of 2^-24 of the row's largest term; terms of dx: rstd (|dh| + |n| mean |dh n|)
+    n = (X * rstd).detach()
+    size = rstd.detach() * (dh.double().abs() + n.abs() * (dh.double() * n).abs().mean(-1, keepdim=True))
+    within(gx, want[0], U[BF16] * want[0].abs() + 128 * 2.0 ** -24 * size, "dx")
+    within(gw, want[1], 128 * 2.0 ** -24 * (dh.double() * n).abs().sum(0), "dw")
