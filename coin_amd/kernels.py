@@ -1149,11 +1149,16 @@ def residual_norm_bwd(x: torch.Tensor, y: Optional[torch.Tensor], gate: Optional
     return (dx, dy, dgate, *params)
 
 
+_SPAN = 2 ** 31 - 1   # byte offsets inside a tile are 32 bits wide in the kernels; the C entry points refuse a tensor whose tiles reach further
+
+
 def chunked_ok(x: torch.Tensor) -> bool:
+    """What coin_linear_* takes as an operand: rows of whole, aligned 16-byte chunks, 260 of them within 2^31 bytes."""
     m, k = x.shape
-    el = 16 // x.element_size()
+    es = x.element_size()
+    el = 16 // es
     s0, s1 = x.stride()
-    return k % el == 0 and s1 == 1 and (m == 1 or (s0 % el == 0 and s0 >= k)) and not x.data_ptr() & 15
+    return k % el == 0 and s1 == 1 and (m == 1 or (s0 % el == 0 and s0 >= k and (260 * s0 + k) * es + 4096 < _SPAN)) and not x.data_ptr() & 15
 
 
 def chunked_rows(x: torch.Tensor) -> torch.Tensor:

@@ -1128,8 +1128,9 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
 
     ``act``: ACT_NONE, ACT_RELU, ACT_GELU (z Phi(z)), ACT_QUICK_GELU (z sigmoid(1.702 z)) or ACT_SILU.  The products run in the compute dtype
     (the autocast dtype, else x's: bfloat16 or float32) with float32 sums; a float32 master weight is read through its bfloat16 shadow and
-    receives a float32 gradient.  ``residual`` [..., N] of the compute dtype, or float32, decides the output's dtype.  Any sizes and strides
-    (rows that are not whole 16-byte chunks are copied first).  Differentiable once in x, weight, bias and residual."""
+    receives a float32 gradient.  ``residual`` [..., N] of the compute dtype, or float32, decides the output's dtype.  Any strides and pitches
+    (rows that are not whole 16-byte chunks, or lie so far apart that 260 of them pass 2^31 bytes, are copied first); K and N up to two
+    million, 2^30 rows.  Differentiable once in x, weight, bias and residual."""
     K._dev(x, weight)
     if act not in (ACT_NONE, ACT_RELU, ACT_GELU, ACT_QUICK_GELU, ACT_SILU):
         raise CoinHipError(f"fused_linear: activation {act}")

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from coin_amd import layers as L
-from test_transformer_ops_gpu import BF16, DEV, F32, U, rand, within
+from test_transformer_ops_gpu import BF16, DEV, F32, U, check_linear, rand, within
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +43,22 @@ def test_gradient_of_an_rms_norm_without_an_epsilon():
     size = rstd.detach() * (dh.double().abs() + n.abs() * (dh.double() * n).abs().mean(-1, keepdim=True))
     within(gx, want[0], U[BF16] * want[0].abs() + 128 * 2.0 ** -24 * size, "dx")
     within(gw, want[1], 128 * 2.0 ** -24 * (dh.double() * n).abs().sum(0), "dw")
+
+
+# ------------------------------------------------------------------------------------------------------------ pitches past 32 bits
+@pytest.mark.parametrize("dtype,rows", [(BF16, 2048), (F32, 1024)])
+def test_linear_on_the_last_token_of_each_sequence(dtype, rows):
+    """x[:, -1] of [3, rows, 2048]: 260 rows of that pitch pass 2^31 bytes, and so they do for a weight and a gradient cut out the same way."""
+    wide = torch.zeros(3, rows, 2048, device=DEV, dtype=dtype)
+    cut = wide[:, -1]
+    cut.copy_(rand((3, 2048), dtype, 1))
+    assert 260 * cut.stride(0) * cut.element_size() >= 2 ** 31
+    for n in (72, 37):
+        check_linear(cut, rand((n, 2048), dtype, 2, 2048 ** -0.5), rand((n,), F32, 3), None, "gelu", f"last tokens, n={n}")
+    check_linear(rand((5, 2048), dtype, 4), cut, None, None, "none", "a weight of wide pitch")
+    x, w = rand((3, 64), dtype, 5).requires_grad_(), rand((2048, 64), dtype, 6, 0.1).requires_grad_()
+    for act in (L.ACT_NONE, L.ACT_SILU):
+        a, b = (torch.autograd.grad(L.fused_linear(x, w, act=act), [x, w], g) for g in (cut, cut.contiguous()))
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    res = wide[:, -1, :72]                                 # the residual is read row by row, whatever its pitch
+    check_linear(rand((3, 64), dtype, 8), rand((72, 64), dtype, 9, 0.1), None, res, "relu", "a residual of wide pitch")
