@@ -962,6 +962,7 @@ class EmaTable:
 # A block's step is a handful of launches of a few microseconds each: what these wrappers do per call is kept small (addresses as plain
 # integers, what depends on shapes and strides alone computed once per shape).
 _WS_CACHE = 1024   # shapes whose workspace sizes are remembered
+_SPAN = 2 ** 31 - 1   # byte offsets inside a tile are 32 bits wide in the kernels; the C entry points refuse a tensor whose tiles reach further
 
 
 def _a(t: Optional[torch.Tensor]):
@@ -1005,14 +1006,17 @@ def _strides(t: torch.Tensor):
     return [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
 
 
-def chunked_heads(t: torch.Tensor) -> torch.Tensor:
-    """`t` [..., D] with whole 16-byte chunks along the last dimension: itself where pointer and strides allow it, else a copy."""
+def chunked_heads(t: torch.Tensor, group: int = 1) -> torch.Tensor:
+    """`t` [B, L, .., H, D] as coin_attention_* takes it -- whole, aligned 16-byte chunks along the last dimension, 130 tokens and the `group`
+    heads that share a key head within 2^31 bytes: itself where pointer and strides allow it, else a copy."""
     if not t.data_ptr() & 15:
-        if t.is_contiguous() and (t.shape[-1] * t.element_size()) & 15 == 0:
-            return t
         es = t.element_size()
-        if t.stride(-1) == 1 and not any(n > 1 and (s * es) & 15 for n, s in zip(t.shape[:-1], t.stride()[:-1])):
+        if t.is_contiguous() and (t.shape[-1] * es) & 15 == 0:
             return t
+        if t.stride(-1) == 1 and not any(n > 1 and (s * es) & 15 for n, s in zip(t.shape[:-1], t.stride()[:-1])):
+            token, head = (t.stride(i) if t.shape[i] > 1 else 0 for i in (1, -2))
+            if (130 * token + group * head) * es < _SPAN:
+                return t
     t = t.contiguous()
     return t.clone() if t.data_ptr() & 15 else t
 
@@ -1020,7 +1024,7 @@ def chunked_heads(t: torch.Tensor) -> torch.Tensor:
 class AttentionPlan:
     """What an attention call's shapes, strides and type decide: checked sizes, the strides of its eight tensors as the C ABI takes them (out
     and the gradients contiguous, or the gradients strided like one [B, L, 3, H, D] tensor), workspace sizes."""
-    __slots__ = ("dims", "code", "strides", "at", "ws_fwd", "ws_bwd", "out_shape", "out_stride", "k_shape")
+    __slots__ = ("dims", "group", "code", "strides", "at", "ws_fwd", "ws_bwd", "out_shape", "out_stride", "k_shape")
 
     def __init__(self, q, k, v, packed: bool):
         if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
@@ -1034,7 +1038,7 @@ class AttentionPlan:
             raise CoinHipError(f"attention: {hq} query heads over {hkv} key heads")
         if d > 128 or d <= 0 or d % (16 // q.element_size()):
             raise CoinHipError(f"attention: head dimension {d} (a multiple of {16 // q.element_size()}, at most 128, for {q.dtype})")
-        self.dims = (b, lq, lk, hq, hkv, d)
+        self.dims, self.group = (b, lq, lk, hq, hkv, d), hq // hkv
         self.out_shape, self.k_shape, self.out_stride = tuple(q.shape), tuple(k.shape), (lq * hq * d, hq * d, d, 1)
         whole = [lq * hq * d, hq * d, d]
         grads = [[3 * lq * hq * d, 3 * hq * d, d]] * 3 if packed else [whole] + [[lk * hkv * d, hkv * d, d]] * 2
@@ -1147,9 +1151,6 @@ def residual_norm_bwd(x: torch.Tensor, y: Optional[torch.Tensor], gate: Optional
             int(rms), scale, stats.data_ptr(), _a(dr), _a(dh), _a(dx), _a(dy), _a(dgate), *map(_a, params), m, d, _code(x.dtype), _code(branch_dtype),
             _code(gate.dtype) if gate is not None else COIN_F32, _a(ws), nbytes)
     return (dx, dy, dgate, *params)
-
-
-_SPAN = 2 ** 31 - 1   # byte offsets inside a tile are 32 bits wide in the kernels; the C entry points refuse a tensor whose tiles reach further
 
 
 def chunked_ok(x: torch.Tensor) -> bool:

@@ -901,7 +901,7 @@ class _Attention(Function):
         q, k, v, out, lo, lse, lengths = ctx.saved_tensors
         plan, dt, dev = ctx.plan, q.dtype, q.device
         dq, dk, dv = (torch.empty(s, dtype=dt, device=dev) for s in (plan.out_shape, plan.k_shape, plan.k_shape))
-        K.attention_bwd(plan, q, k, v, out, lo, K.chunked_heads(dout), lse, ctx.causal, ctx.scale, lengths, dq, dk, dv)
+        K.attention_bwd(plan, q, k, v, out, lo, K.chunked_heads(dout, plan.group), lse, ctx.causal, ctx.scale, lengths, dq, dk, dv)
         return dq, dk, dv, None, None, None, None
 
 
@@ -948,7 +948,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     K._dev(q, k, v)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     lengths = _lengths32(key_lengths)
-    q, k, v = K.chunked_heads(q), K.chunked_heads(k), K.chunked_heads(v)
+    q, k, v = K.chunked_heads(q, q.shape[2] // max(k.shape[2], 1)), K.chunked_heads(k), K.chunked_heads(v)
     plan = K.attention_plan(q, k, v)
     if _wants_grad(q, k, v):
         return _Attention.apply(q, k, v, lengths, bool(causal), scale, plan)

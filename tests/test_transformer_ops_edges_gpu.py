@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from coin_amd import layers as L
-from test_transformer_ops_gpu import BF16, DEV, F32, U, check_linear, rand, within
+from test_transformer_ops_gpu import BF16, DEV, F32, U, check_attention, check_linear, rand, within
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,35 @@ def test_linear_on_the_last_token_of_each_sequence(dtype, rows):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
     res = wide[:, -1, :72]                                 # the residual is read row by row, whatever its pitch
     check_linear(rand((3, 64), dtype, 8), rand((72, 64), dtype, 9, 0.1), None, res, "relu", "a residual of wide pitch")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_over_tokens_that_lie_far_apart(dtype):
+    pitch = 2 ** 31 // (130 * (2 if dtype == BF16 else 4)) // 64 * 64 + 128
+
+    def apart(n, heads, seed):
+        base = torch.empty(n, pitch, device=DEV, dtype=dtype)
+        t = base[:, :heads * 64].unflatten(1, (heads, 64))[None]
+        t.copy_(rand(t.shape, dtype, seed))
+        return t
+
+    q, k, v = rand((1, 9, 4, 64), dtype, 1), apart(7, 2, 2), apart(7, 2, 3)
+    check_attention(q, k, v, True, None, "keys far apart")
+    check_attention(apart(9, 4, 4), k.contiguous(), v, False, torch.tensor([5], device=DEV, dtype=torch.int32), "queries far apart")
+    qq, kk, vv = (t.contiguous().requires_grad_() for t in (q, k, v))
+    dout = apart(9, 4, 5)
+    a, b = (torch.autograd.grad(L.attention(qq, kk, vv), [qq, kk, vv], g) for g in (dout, dout.contiguous()))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_attention_over_heads_that_lie_far_apart():
+    """Four query heads of one key head, 2^29 bytes from one another: the gradients walk them as rows of one product."""
+    base = torch.empty(4, 1 << 28, device=DEV, dtype=BF16)
+    q = base[:, :9 * 64].unflatten(1, (9, 64)).transpose(0, 1)[None]
+    q.copy_(rand((1, 9, 4, 64), BF16, 1))
+    assert q.stride(2) == 1 << 28
+    k, v = rand((1, 40, 1, 64), BF16, 2), rand((1, 40, 1, 64), BF16, 3)
+    check_attention(q, k, v, True, None, "heads far apart")
+    qq = q.contiguous().requires_grad_()
+    a, b = (torch.autograd.grad(L.attention(qq, k, v), qq, g)[0] for g in (q, q.contiguous()))
+    assert torch.equal(a, b)
