@@ -9,7 +9,7 @@ import weakref
 from typing import Optional, Sequence, Tuple
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import kernels as K
@@ -883,8 +883,15 @@ def rpn_losses(logits, deltas, labels, anchors, matched_gt, min_label=0):
 
 
 # --------------------------------------------------------------------------- transformer blocks
-def _wants_grad(*ts: Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+def _needs_function(*ts: Optional[torch.Tensor]) -> bool:
+    """Must the call go through its `Function`?  For a gradient, and inside a forward-mode level: the `Function` refuses operands with a
+    tangent, which a launch on bare pointers would drop."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)) or forward_ad._current_level >= 0
+
+
+def _not_traced(what: str) -> None:
+    if torch.jit.is_tracing():
+        raise CoinHipError(f"{what}: torch.jit.trace would keep this call's sizes for every other, or record nothing of it")
 
 
 class _Attention(Function):
@@ -943,6 +950,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     keys is Lq = 1.  A query that sees no key gives zeros.  Inside the keys a query may be compared with, values must be finite: masked
     ones enter the products with a weight of zero.  D: a multiple of 8 (bfloat16) or 4 (float32), at most 128.  Differentiable once in
     q, k and v; ``scale`` is 1 / sqrt(D) where it is not given."""
+    _not_traced("attention")
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise CoinHipError("attention: q, k and v are [B, L, H, D]")
     K._dev(q, k, v)
@@ -950,7 +958,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     lengths = _lengths32(key_lengths)
     q, k, v = K.chunked_heads(q, q.shape[2] // max(k.shape[2], 1)), K.chunked_heads(k), K.chunked_heads(v)
     plan = K.attention_plan(q, k, v)
-    if _wants_grad(q, k, v):
+    if _needs_function(q, k, v):
         return _Attention.apply(q, k, v, lengths, bool(causal), scale, plan)
     return K.attention_fwd(plan, q, k, v, causal, scale, lengths)[0]
 
@@ -959,6 +967,7 @@ def attention_qkv(qkv: torch.Tensor, heads: int, *, causal: bool = False, scale:
                   key_lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
     """`attention` of one sequence's tokens among themselves on the projection qkv [B, L, 3 * heads * D] ([3][heads][D] along the last axis)
     -> [B, L, heads * D]; one gradient of qkv's layout."""
+    _not_traced("attention_qkv")
     K._dev(qkv)
     if qkv.dim() != 3 or heads <= 0 or qkv.shape[2] % (3 * heads):
         raise CoinHipError(f"attention_qkv: [B, L, 3 * {heads} * D] expected, got {tuple(qkv.shape)}")
@@ -969,7 +978,7 @@ def attention_qkv(qkv: torch.Tensor, heads: int, *, causal: bool = False, scale:
     lengths = _lengths32(key_lengths)
     q, k, v = x.unbind(2)
     plan = K.attention_plan(q, k, v, packed=True)
-    if _wants_grad(x):
+    if _needs_function(x):
         out = _AttentionQKV.apply(x, lengths, bool(causal), scale, plan)
     else:
         out = K.attention_fwd(plan, q, k, v, causal, scale, lengths)[0]
@@ -1030,6 +1039,7 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_nor
     dimensions followed by ones and D (a gate for each sequence), float32 or bfloat16.  Streams are float32 or bfloat16; branches (y and h)
     float32 or bfloat16, bfloat16 on a bfloat16 stream; ``branch_dtype`` (default: y's, else the compute dtype) is h's.  h is the norm of r
     before r is rounded to the stream's type.  D at most 8192.  Differentiable once in x, y, gate and the norms' parameters."""
+    _not_traced("residual_norm")
     K._dev(x)
     d = x.shape[-1] if x.dim() else 0
     if x.dim() < 1 or d < 1 or d > 8192:
@@ -1080,7 +1090,7 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_nor
         return r, None if pre_norm is None else r.to(branch_dtype) * 1.0 + (zero.to(branch_dtype) if torch.is_tensor(zero) else zero)
     x, y, gate = (t if t is None or t.is_contiguous() else t.contiguous() for t in (x, y, gate))
     rms = True in kinds
-    if _wants_grad(x, y, gate, pw, pb, nw, nb):
+    if _needs_function(x, y, gate, pw, pb, nw, nb):
         r, h = _ResidualNorm.apply(x, y, gate, pw, pb, nw, nb, (rows_per_gate, post_eps, pre_eps, rms, float(scale), branch_dtype))
     else:
         post, pre = (pw, pb, post_eps) if post_norm is not None else None, (nw, nb, pre_eps) if pre_norm is not None else None
@@ -1131,6 +1141,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     receives a float32 gradient.  ``residual`` [..., N] of the compute dtype, or float32, decides the output's dtype.  Any strides and pitches
     (rows that are not whole 16-byte chunks, or lie so far apart that 260 of them pass 2^31 bytes, are copied first); K and N up to two
     million, 2^30 rows.  Differentiable once in x, weight, bias and residual."""
+    _not_traced("fused_linear")
     K._dev(x, weight)
     if act not in (ACT_NONE, ACT_RELU, ACT_GELU, ACT_QUICK_GELU, ACT_SILU):
         raise CoinHipError(f"fused_linear: activation {act}")
@@ -1160,7 +1171,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         return out if residual is None else residual + out.to(residual.dtype)
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    if _wants_grad(x, weight, bias, residual):
+    if _needs_function(x, weight, bias, residual):
         return _FusedLinear.apply(x, weight, bias, residual, wq.detach(), act)
     r2 = _rows(residual) if residual is not None else None
     return K.linear_fwd(K.chunked_rows(_rows(x)), K.chunked_rows(wq), k, bias, act, r2, dt if r2 is None else r2.dtype, False)[0].view(shape)

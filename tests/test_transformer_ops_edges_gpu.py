@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from coin_amd import layers as L
+from coin_amd._lib import CoinHipError
 from test_transformer_ops_gpu import BF16, DEV, F32, U, check_attention, check_linear, rand, within
 
 pytestmark = pytest.mark.gpu
@@ -94,3 +95,44 @@ def test_attention_over_heads_that_lie_far_apart():
     qq = q.contiguous().requires_grad_()
     a, b = (torch.autograd.grad(L.attention(qq, k, v), qq, g)[0] for g in (q, q.contiguous()))
     assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------------- forward mode and recorded calls
+def calls():
+    """One call of each entry point as a function of one tensor, and that tensor."""
+    w, ln = rand((16, 16), F32, 5), torch.nn.LayerNorm(16, device=DEV).requires_grad_(False)
+    kv = rand((2, 7, 2, 8), F32, 6)
+    x = rand((3, 16), F32, 7)
+    return {
+        "attention": (lambda t: L.attention(t, kv, kv), rand((2, 5, 4, 8), F32, 1)),
+        "attention keys": (lambda t: L.attention(kv, t, kv), rand((2, 7, 2, 8), F32, 1)),
+        "attention_qkv": (lambda t: L.attention_qkv(t, 2), rand((2, 5, 48), F32, 2)),
+        "residual_norm": (lambda t: L.residual_norm(x, t, pre_norm=ln)[1], rand((3, 16), F32, 3)),
+        "fused_linear": (lambda t: L.fused_linear(t, w, act=L.ACT_GELU), rand((3, 16), F32, 4)),
+        "fused_linear weight": (lambda t: L.fused_linear(x, t), rand((16, 16), F32, 4)),
+    }
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_forward_mode_tangent_is_refused_not_dropped(grad):
+    for name, (f, t) in calls().items():
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+            assert not dual.requires_grad
+            with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                f(dual)
+                pytest.fail(f"{name} gave a result without its tangent")
+            with torch.no_grad():
+                assert torch.equal(f(t), f(t.clone())), name          # operands without a tangent are as good as outside
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (t,), (torch.ones_like(t),))
+            pytest.fail(f"{name} gave a result without its tangent")
+
+
+def test_a_traced_call_is_refused():
+    for name, (f, t) in calls().items():
+        for needs in (False, True):
+            with pytest.raises(CoinHipError):
+                torch.jit.trace(f, (t.detach().clone().requires_grad_(needs),), check_trace=False)
+                pytest.fail(f"{name} was recorded")
+        assert f(t).isfinite().all()
