@@ -894,6 +894,14 @@ def _not_traced(what: str) -> None:
         raise CoinHipError(f"{what}: torch.jit.trace would keep this call's sizes for every other, or record nothing of it")
 
 
+def calls_only(module: torch.nn.Module, *kinds: type) -> bool:
+    """Would calling `module` run the forward of one of the classes `kinds` and nothing else: no forward of its own, no hooks?  What uses a module's
+    parameters without calling it must give the same, and skip nothing that a user attached."""
+    return (any(isinstance(module, k) and type(module).forward is k.forward for k in kinds) and "forward" not in module.__dict__
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
+            and not torch.nn.modules.module._has_any_global_hook())
+
+
 class _Attention(Function):
     @staticmethod
     def forward(ctx, q, k, v, key_lengths, causal, scale, plan):

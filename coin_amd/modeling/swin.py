@@ -93,7 +93,8 @@ def shift_mask(hp: int, wp: int, ws: int, shift: int, device) -> torch.Tensor:
 
 class SwinBlock(nn.Module):
     """``fused`` (cfg.AMD.FUSED_BLOCKS): on the device the norms and the residual add run on `L.residual_norm`, the linear layers with their
-    activation and residual on `L.fused_linear`; the same formulas, rounded in other places."""
+    activation and residual on `L.fused_linear`; the same formulas, rounded in other places.  A block whose norms carry hooks, or were replaced,
+    calls them as it does without."""
 
     def __init__(self, dim: int, heads: int, window: int, shift: int, mlp_ratio: float = 4.0, fused: bool = False):
         super().__init__()
@@ -120,7 +121,7 @@ class SwinBlock(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:  # [N, H, W, C]
         n, h, w, c = x.shape
         ws, t = self.window, self.window * self.window
-        fused = self.fused and x.is_cuda
+        fused = self.fused and x.is_cuda and L.calls_only(self.norm1, nn.LayerNorm) and L.calls_only(self.norm2, nn.LayerNorm)
         linear = L.fused_linear if fused else L.linear
         y = L.residual_norm(x, pre_norm=self.norm1)[1] if fused else self.norm1(x)
         ph, pw = (-h) % ws, (-w) % ws

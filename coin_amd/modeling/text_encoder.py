@@ -50,7 +50,7 @@ class _Attention(nn.Module):
 
 class ResidualAttentionBlock(nn.Module):
     """``fused`` (cfg.AMD.FUSED_BLOCKS): on the device the block runs on `L.attention_qkv`, `L.residual_norm` and `L.fused_linear`; the same
-    formulas, rounded in other places."""
+    formulas, rounded in other places.  A block whose norms or attention carry hooks, or were replaced, calls them as it does without."""
 
     def __init__(self, d: int, heads: int, fused: bool = False):
         super().__init__()
@@ -61,7 +61,7 @@ class ResidualAttentionBlock(nn.Module):
         self.ln_2 = nn.LayerNorm(d)
 
     def forward(self, x):
-        if self.fused and x.is_cuda:
+        if self.fused and x.is_cuda and L.calls_only(self.attn, _Attention) and L.calls_only(self.ln_1, nn.LayerNorm) and L.calls_only(self.ln_2, nn.LayerNorm):
             a, fc, pr = self.attn, self.mlp.c_fc, self.mlp.c_proj
             _, h = L.residual_norm(x, pre_norm=self.ln_1)
             y = L.attention_qkv(L.fused_linear(h, a.in_proj_weight, a.in_proj_bias), a.heads, causal=True)
