@@ -894,12 +894,16 @@ def _not_traced(what: str) -> None:
         raise CoinHipError(f"{what}: torch.jit.trace would keep this call's sizes for every other, or record nothing of it")
 
 
-def calls_only(module: torch.nn.Module, *kinds: type) -> bool:
-    """Would calling `module` run the forward of one of the classes `kinds` and nothing else: no forward of its own, no hooks?  What uses a module's
-    parameters without calling it must give the same, and skip nothing that a user attached."""
+def _is_plain(module: Optional[torch.nn.Module], *kinds: type) -> bool:
+    """Is `module`'s forward that of one of the classes `kinds`, without hooks of its own that could change what it takes, holds or gives?"""
     return (any(isinstance(module, k) and type(module).forward is k.forward for k in kinds) and "forward" not in module.__dict__
-            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
-            and not torch.nn.modules.module._has_any_global_hook())
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+
+
+def calls_only(module: torch.nn.Module, *kinds: type) -> bool:
+    """Would calling `module` run the forward of one of the classes `kinds` and nothing else?  What uses a module's parameters without calling it
+    must give the same, and skip nothing that a user attached."""
+    return _is_plain(module, *kinds) and not torch.nn.modules.module._has_any_global_hook()
 
 
 class _Attention(Function):
@@ -1029,8 +1033,8 @@ class _ResidualNorm(Function):
 
 def _norm_of(norm: Optional[torch.nn.Module], d: int):
     """(weight, bias, eps, is it an RMSNorm) of an nn.LayerNorm / nn.RMSNorm over rows of d."""
-    if not isinstance(norm, (torch.nn.LayerNorm, torch.nn.RMSNorm)) or tuple(norm.normalized_shape) != (d,):
-        raise CoinHipError(f"residual_norm: nn.LayerNorm({d}) or nn.RMSNorm({d}) expected, got {norm}")
+    if not _is_plain(norm, torch.nn.LayerNorm, torch.nn.RMSNorm) or tuple(norm.normalized_shape) != (d,):
+        raise CoinHipError(f"residual_norm: nn.LayerNorm({d}) or nn.RMSNorm({d}) without hooks or a forward of its own expected, got {norm}")
     rms = isinstance(norm, torch.nn.RMSNorm)
     f32 = lambda p: None if p is None else (p if p.dtype == torch.float32 else p.float()).contiguous()  # noqa: E731
     # an RMSNorm without an epsilon: the module computes bfloat16 rows in float32 too and takes that type's
@@ -1043,10 +1047,11 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_nor
     """r = x + scale * gate * post_norm(y);  h = pre_norm(r).  -> (r, h), h None without ``pre_norm``; without ``y``, r is x.
 
     The end of one branch of a transformer block and the start of the next in one pass: x [..., D] the residual stream, y the branch's
-    output, ``pre_norm`` / ``post_norm`` nn.LayerNorm(D) or nn.RMSNorm(D) modules of one kind.  ``gate``: [D] (a layer scale), or x's leading
-    dimensions followed by ones and D (a gate for each sequence), float32 or bfloat16.  Streams are float32 or bfloat16; branches (y and h)
-    float32 or bfloat16, bfloat16 on a bfloat16 stream; ``branch_dtype`` (default: y's, else the compute dtype) is h's.  h is the norm of r
-    before r is rounded to the stream's type.  D at most 8192.  Differentiable once in x, y, gate and the norms' parameters."""
+    output, ``pre_norm`` / ``post_norm`` nn.LayerNorm(D) or nn.RMSNorm(D) modules of one kind, which are not called: one with hooks, or a
+    subclass with a forward of its own, is refused.  ``gate``: [D] (a layer scale), or x's leading dimensions followed by ones and D (a gate
+    for each sequence), float32 or bfloat16.  Streams are float32 or bfloat16; branches (y and h) float32 or bfloat16, bfloat16 on a
+    bfloat16 stream; ``branch_dtype`` (default: y's, else the compute dtype) is h's.  h is the norm of r before r is rounded to the
+    stream's type.  D at most 8192.  Differentiable once in x, y, gate and the norms' parameters."""
     _not_traced("residual_norm")
     K._dev(x)
     d = x.shape[-1] if x.dim() else 0

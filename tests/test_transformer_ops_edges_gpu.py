@@ -2,6 +2,7 @@
 default epsilons, wide pitches, column sums, rows that the mask leaves empty, infinities and NaN, forward-mode derivatives."""
 import pytest
 import torch
+import torch.nn.utils.parametrize
 
 from coin_amd import layers as L
 from coin_amd._lib import CoinHipError
@@ -136,3 +137,37 @@ def test_a_traced_call_is_refused():
                 torch.jit.trace(f, (t.detach().clone().requires_grad_(needs),), check_trace=False)
                 pytest.fail(f"{name} was recorded")
         assert f(t).isfinite().all()
+
+
+# -------------------------------------------------------------------------------------------------- modules that are not what they seem
+class _Shifted(torch.nn.LayerNorm):
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+class _Named(torch.nn.RMSNorm):
+    """A subclass that computes what its base does."""
+
+
+def test_norms_that_compute_something_else_are_refused():
+    x, y = rand((4, 16), F32, 1), rand((4, 16), F32, 2)
+    swapped = torch.nn.LayerNorm(16, device=DEV)
+    swapped.forward = lambda t: t
+    hooked = [torch.nn.LayerNorm(16, device=DEV) for _ in range(3)]
+    hooked[0].register_forward_hook(lambda m, i, o: 2 * o)
+    hooked[1].register_forward_pre_hook(lambda m, i: (2 * i[0],))
+    hooked[2].register_full_backward_hook(lambda m, gi, go: None)
+    for bad in [_Shifted(16, device=DEV), swapped] + hooked:
+        for kw in (dict(pre_norm=bad), dict(post_norm=bad)):
+            with pytest.raises(CoinHipError):
+                L.residual_norm(x, y, **kw)
+                pytest.fail(f"{bad} was taken for its base")
+    a, b = _Named(16, device=DEV), torch.nn.RMSNorm(16, device=DEV)
+    assert torch.equal(L.residual_norm(x, y, pre_norm=a)[1], L.residual_norm(x, y, pre_norm=b)[1])
+    torch.nn.utils.parametrize.register_parametrization(b, "weight", _Doubled())
+    within(L.residual_norm(x, pre_norm=b)[1], 2 * L.residual_norm(x, pre_norm=a)[1].detach().double(), 2.0 ** -30 * torch.ones_like(x).double(), "parametrized")
+
+
+class _Doubled(torch.nn.Module):
+    def forward(self, w):
+        return 2 * w
