@@ -6,6 +6,7 @@ import torch.nn.utils.parametrize
 
 from coin_amd import layers as L
 from coin_amd._lib import CoinHipError
+from norm_oracle import residual_norm64
 from test_transformer_ops_gpu import BF16, DEV, F32, U, check_attention, check_linear, rand, within
 
 pytestmark = pytest.mark.gpu
@@ -171,3 +172,39 @@ def test_norms_that_compute_something_else_are_refused():
 class _Doubled(torch.nn.Module):
     def forward(self, w):
         return 2 * w
+
+
+# ------------------------------------------------------------------------------------------------------------------ sums over the rows
+WALKS = [   # rows of one gate: over many walks of the backward, a part of one, several whole ones within one, one row each
+    ((5, 1000), 64), ((1000, 5), 64), ((3000, 1), 32), ((700, 9), 520), ((40000, 3), 32), ((4500, 2), 2501), ((9, 77), 512), ((2, 37), 96), ((40, 130), 16),
+    ((700,), 136), ((3, 41), 768), ((7, 9), 100), ((3, 500), 4096), ((2, 700), 8192),
+]
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (F32, BF16), (BF16, BF16)])
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("lead,d", WALKS)
+def test_residual_norm_gradients_column_by_column(lead, d, rms, types):
+    """Both norms and a gate, by layer and by group; every gradient within the bounds of norm_oracle, which are asserted to be a small part of
+    the sums (a walk's rows are added one by one, then 16 walks, up to 64 + 16 workgroups: 128 levels while a walk has up to 32 rows)."""
+    ts, tb = types
+    kind = torch.nn.RMSNorm if rms else torch.nn.LayerNorm
+    post, pre = kind(d, eps=1e-5, device=DEV), kind(d, eps=1e-5, device=DEV)
+    with torch.no_grad():
+        for i, p in enumerate(list(post.parameters()) + list(pre.parameters())):
+            p.mul_(1.0).add_(rand((d,), F32, 20 + i, 0.3))
+    x, y = rand(lead + (d,), ts, 1).requires_grad_(), rand(lead + (d,), tb, 2).requires_grad_()
+    dr, dh = rand(lead + (d,), ts, 3), rand(lead + (d,), tb, 4)
+    for groups in (False, True):
+        gate = rand(lead[:1] + (1,) * (len(lead) - 1) + (d,) if groups else (d,), tb if groups else F32, 5, 0.5).requires_grad_()
+        outs = L.residual_norm(x, y, post_norm=post, gate=gate, scale=0.7, pre_norm=pre)
+        leaves = {"dx": x, "dy": y, "dgate": gate, **{f"d{w}_{n}": p for w, m in (("post", post), ("pre", pre)) for n, p in m.named_parameters()}}
+        got = dict(zip(leaves, torch.autograd.grad(outs, list(leaves.values()), [dr, dh])), r=outs[0].detach(), h=outs[1].detach())
+        par = lambda m: (m.weight, getattr(m, "bias", None) if not rms else 0.0, 1e-5)  # noqa: E731
+        want = residual_norm64(x, y, par(post), gate, 0.7, par(pre), rms, dr, dh, depth=128, groups=groups)
+        for name, t in got.items():
+            value, bound, terms = want[name]
+            if name.startswith(("dgate", "dpost", "dpre")):
+                # worst cases of m terms add up with m, terms of random signs with its root: 120000 rows leave the largest ratio
+                assert bool((bound < 0.1 * value.abs().amax()).all()), name
+            within(t, value, bound + (U[t.dtype] * value.abs() if t.dtype == BF16 else 2 * U[F32] * value.abs()), f"{name}, groups={groups}")
