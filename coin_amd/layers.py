@@ -959,9 +959,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
 
     ``key_lengths`` [B]: sequence b has its first n_b keys only (what lies behind them does not matter; their gradients are zeros).
     ``causal``: query i sees the keys j <= i + n_b - Lq, so the last query sees the whole sequence -- a single new token over a cache of
-    keys is Lq = 1.  A query that sees no key gives zeros.  Inside the keys a query may be compared with, values must be finite: masked
-    ones enter the products with a weight of zero.  D: a multiple of 8 (bfloat16) or 4 (float32), at most 128.  Differentiable once in
-    q, k and v; ``scale`` is 1 / sqrt(D) where it is not given."""
+    keys is Lq = 1.  A query that sees no key gives zeros, whatever it holds.  Inside the keys a query may be compared with, values must be
+    finite: masked ones enter the products with a weight of zero.  D: a multiple of 8 (bfloat16) or 4 (float32), at most 128.
+    Differentiable once in q, k and v; ``scale`` is 1 / sqrt(D) where it is not given."""
     _not_traced("attention")
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise CoinHipError("attention: q, k and v are [B, L, H, D]")

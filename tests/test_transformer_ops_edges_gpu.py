@@ -7,7 +7,7 @@ import torch.nn.utils.parametrize
 from coin_amd import layers as L
 from coin_amd._lib import CoinHipError
 from norm_oracle import residual_norm64
-from test_transformer_ops_gpu import BF16, DEV, F32, U, check_attention, check_linear, rand, within
+from test_transformer_ops_gpu import BF16, DEV, F32, U, attention_oracle, check_attention, check_linear, rand, within
 
 pytestmark = pytest.mark.gpu
 
@@ -208,3 +208,79 @@ def test_residual_norm_gradients_column_by_column(lead, d, rms, types):
                 # worst cases of m terms add up with m, terms of random signs with its root: 120000 rows leave the largest ratio
                 assert bool((bound < 0.1 * value.abs().amax()).all()), name
             within(t, value, bound + (U[t.dtype] * value.abs() if t.dtype == BF16 else 2 * U[F32] * value.abs()), f"{name}, groups={groups}")
+
+
+# ------------------------------------------------------------------------------------------------------------------ infinities and NaN
+@pytest.mark.parametrize("types", [(F32, F32), (F32, BF16), (BF16, BF16)])
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("d", [40, 100, 2048])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_residual_norm_keeps_a_bad_row_to_itself(bad, d, rms, types):
+    """One bad value in x, y, dr or dh: rows without it keep their bits, its own row is not finite wherever the definition's is not, and so are the
+    sums it enters: all columns' or its own, and its own group's gate alone."""
+    ts, tb = types
+    kind = torch.nn.RMSNorm if rms else torch.nn.LayerNorm
+    post, pre = kind(d, eps=1e-5, device=DEV), kind(d, eps=1e-5, device=DEV)
+    lead, at = (6, 11), (2, 7)
+    base = [rand(lead + (d,), t, i) for i, t in enumerate((ts, tb, ts, tb))]
+    gate = rand((6, 1, d), tb, 9, 0.5)
+    rows = torch.ones(lead, dtype=torch.bool, device=DEV)
+    rows[at] = False
+
+    def run(ts_, f):
+        x, y, g = (t.detach().requires_grad_() for t in (ts_[0], ts_[1], gate.double() if f is plain else gate))
+        leaves = [x, y, g] + list(post.parameters()) + list(pre.parameters())
+        outs = f(x, y, g)
+        return [t.detach() for t in outs] + list(torch.autograd.grad(outs, leaves, [t.to(o.dtype) for t, o in zip(ts_[2:], outs)]))
+
+    def own(x, y, g):
+        return L.residual_norm(x, y, post_norm=post, gate=g, scale=0.5, pre_norm=pre)
+
+    def plain(x, y, g):
+        def norm(t, m):
+            c = t if rms else t - t.mean(-1, keepdim=True)
+            return c * (c.pow(2).mean(-1, keepdim=True) + 1e-5).rsqrt() * m.weight.double() + (0.0 if rms else m.bias.double())
+        r = x.double() + 0.5 * g * norm(y.double(), post)
+        return r, norm(r, pre)
+
+    clean = run(base, own)
+    for i in range(4):
+        ts_ = [t.clone() for t in base]
+        ts_[i][at + (3,)] = bad
+        got, want = run(ts_, own), run(ts_, plain)
+        for j in (0, 1, 2, 3):                                                   # r, h, dx, dy
+            assert torch.equal(got[j][rows], clean[j][rows]), (i, j)
+            assert not (got[j].isfinite() & ~want[j].isfinite()).any(), (i, j)    # nothing bad is made good
+            assert bool(got[j][want[j].isfinite()].isfinite().all()), (i, j)      # nor the other way
+        other = [k for k in range(6) if k != at[0]]
+        assert torch.equal(got[4][other], clean[4][other])
+        for g, w in zip(got[4:], want[4:]):
+            assert torch.equal(g.isfinite(), w.isfinite()), i
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(2, 70, 30, 4, 2, 64), (1, 300, 170, 2, 1, 128), (1, 900, 40, 2, 2, 32)])
+def test_queries_that_see_no_key_may_hold_anything(shape, dtype):
+    """More causal queries than keys: the first rows see nothing.  NaN in them and in their gradient reaches no other result."""
+    b, lq, lk, hq, hkv, d = shape
+    q, k, v = rand((b, lq, hq, d), dtype, 1), rand((b, lk, hkv, d), dtype, 2), rand((b, lk, hkv, d), dtype, 3)
+    n = torch.tensor([lk - 3 * i for i in range(b)], device=DEV, dtype=torch.int32)
+    dout = rand(q.shape, dtype, 4)
+    dead = torch.arange(lq, device=DEV)[None, :] < lq - n[:, None]
+    qb, gb = q.clone(), dout.clone()
+    qb[dead] = float("nan")
+    gb[dead] = float("nan")
+    res = []
+    for qq, gg in ((q, dout), (qb, gb)):
+        ts = [t.clone().requires_grad_() for t in (qq, k, v)]
+        out = L.attention(*ts, causal=True, key_lengths=n)
+        with torch.no_grad():
+            again = L.attention(*ts, causal=True, key_lengths=n)
+        res.append([out.detach(), again] + list(torch.autograd.grad(out, ts, gg)))
+    zero = torch.where(dead[:, :, None, None], torch.zeros_like(dout), dout)
+    ref = attention_oracle(q, k, v, True, d ** -0.5, n, zero)
+    for name, clean, bad in zip(("out", "out", "dq", "dk", "dv"), *res):
+        assert not clean.isnan().any()
+        within(bad, *ref[name], name)
+        if name in ("out", "dq"):
+            assert not bad[dead].any(), name
