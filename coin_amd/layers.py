@@ -896,8 +896,11 @@ def _not_traced(what: str) -> None:
 
 def _is_plain(module: Optional[torch.nn.Module], *kinds: type) -> bool:
     """Is `module`'s forward that of one of the classes `kinds`, without hooks of its own that could change what it takes, holds or gives?"""
-    return (any(isinstance(module, k) and type(module).forward is k.forward for k in kinds) and "forward" not in module.__dict__
-            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+    t = type(module)
+    if t not in kinds and not any(issubclass(t, k) and t.forward is k.forward for k in kinds):
+        return False
+    d = module.__dict__
+    return not (d["_forward_hooks"] or d["_forward_pre_hooks"] or d["_backward_hooks"] or d["_backward_pre_hooks"] or "forward" in d)
 
 
 def calls_only(module: torch.nn.Module, *kinds: type) -> bool:
