@@ -132,8 +132,9 @@ struct Cfg {
 
 // ------------------------------------------------------------------------------------------------------------------------------ forward
 // 128 rows by four waves, or up to 32 rows by one; a wave's 32 rows keep Q (32 registers at D 128), the scores of 64 keys (32) and O (64) within
-// the 256 that let two waves on a SIMD (workgroups of one wave, each with its own tiles: 480 us instead of 199 on the long case below, one card).
-// Bound by issue: on that case the matrix units are busy 49 % of the SIMDs' cycles and vector instructions (exponentials, sums, conversions and the
+// the 256 that let two waves on a SIMD (workgroups of one wave, each with its own tiles, take 2.4 times as long on the long case below).
+// Bound by issue as it stands (a tile's scores, its exponentials and its second product follow one another within a wave): on that case the
+// matrix units are busy 49 % of the SIMDs' cycles and vector instructions (exponentials, sums, conversions and the
 // issue of the products) 47 %, with two waves to cover one another.
 // 2 x 4001 causal tokens, 16 heads over 4, D 128, bfloat16: 179 us, 732 TFLOP/s.  One row per sequence over a long cache is bound by memory:
 // 16 ragged caches of up to 32768 keys, 276 us at 4.1 TB/s.
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) voi
   for (int d = 0; d < C::ND; ++d) o[d] = zero16();
   // l: the sum that L is made of.  lw[0]: the sum of the rounded probabilities that the product takes; o = sum p~ v / sum p~ is off by the
   // roundings times (v_j - o) instead of v_j, which is what D and through it dQ and dK see.  It comes from the matrix units, as one more row
-  // of V^T that holds ones: the vector unit is the busier one (198 -> 191 us on the long case, one card)
+  // of V^T that holds ones: the vector unit is the busier one (3.5 % of the long case's time)
   float m = -INFINITY, l = 0.f;
   f32x16 lw = zero16();
   const float c = p.c;
@@ -452,8 +453,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void at
   using C = Cfg<T, DP>;
   constexpr int NW = 4;
   // D 128: the fragments of K (32 registers in bfloat16, 64 in float32), of V (as many) and the two accumulators (128) leave too little of 256 or
-  // 512 registers.  With V in LDS and no spill: 2 x 4001 causal tokens, bfloat16, 401 -> 390 us (one card; V's 32 KiB beside tiles of 32 rows still
-  // let two workgroups on a CU); 4000 causal tokens, 32 heads over 8, float32, 2919 -> 2478 us.  Four waves at any size: workgroups of one wave took
+  // 512 registers.  With V in LDS and no spill: 2 x 4001 causal tokens, bfloat16, 3 % faster (V's 32 KiB beside tiles of 32 rows still let
+  // two workgroups on a CU); 4000 causal tokens, 32 heads over 8, float32, 2919 -> 2478 us.  Four waves at any size: workgroups of one wave took
   // 347 us instead of 133 ([2 x 2001], 16 heads over 4, D 128, causal, bfloat16), and as long where there are few tokens
   constexpr bool VL = DP == 128;
   constexpr int ROWB = C::ROWB, KT = VL ? 32 : C::KT, NS = KT / 32;
@@ -644,8 +645,8 @@ constexpr int64_t SPAN = 0x7fffffff;
 static int cus() { return 256; }   // MI355X
 
 // Keys per split of the forward.  Up to 32 rows (a few tokens over a cache): one wave a workgroup, 8 workgroups a CU where fewer than 2 a CU
-// would run.  Measured on one token over 16 ragged caches of up to 32768 keys, 32 heads over 8: 4 workgroups a CU 294 + 6 us of joining, 8
-// 289 + 11, 16 298 + 18; the lengths are ragged, so the finer of the two that tie.  More rows: four waves, 4 workgroups a CU where fewer than
+// would run.  Measured on one token over 16 ragged caches of up to 32768 keys, 32 heads over 8, join included: 4 workgroups a CU take as
+// long as 8, 16 take 5 % longer; the lengths are ragged, so the finer of the two that tie.  More rows: four waves, 4 workgroups a CU where fewer than
 // one would run.  [1 x 16000] tokens, one head of 128, bfloat16: 277 us with one-wave workgroups in 5 splits, 123 with four waves in 9;
 // [1 x 500] over 20000 keys, 8 heads of 64: 74, 55; float32 [1 x 2048], 8 heads over 2 of 64: 152 unsplit, 99.  Pieces under 256 keys would pay
 // more for the join than they gain
@@ -663,8 +664,8 @@ static int fwd_splits(int64_t wgs, int waves, int Lk, int* chunk) {
 
 // Row splits of the dK, dV launch: its workgroups (128 keys of a head) run two to a CU (D 128 float32: one), and a causal head's are unequal, so
 // two rounds' worth are wanted while there are 512 rows for each; where half the chip would idle, one round's worth down to 128 rows each.
-// 2 x 4001 causal tokens, 16 heads over 4, D 128 (256 workgroups unsplit): no split 976 us, two 563 + 15 us of joining, four 390 + 25, eight
-// 410 + 45.  [1 x 1000], 8 heads of 64 (64 workgroups): unsplit 42 us, 7 splits 23 with the join; [4 x 333], 16 heads of 128 (192): unsplit 29, two 36
+// 2 x 4001 causal tokens, 16 heads over 4, D 128 (256 workgroups unsplit), join included, relative to four splits: none 2.35, two 1.39, eight
+// 1.10.  [1 x 1000], 8 heads of 64 (64 workgroups): unsplit 42 us, 7 splits 23 with the join; [4 x 333], 16 heads of 128 (192): unsplit 29, two 36
 static int dkv_splits(int64_t wgs, int64_t R) {
   if (wgs <= 0) return 1;
   int64_t s = (4 * cus() + wgs - 1) / wgs, fill = 2 * wgs <= cus() ? 2 * cus() / wgs : 1;

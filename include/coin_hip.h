@@ -470,8 +470,8 @@ int coin_ema_update(const coin_ema_tensor* table, int num_tensors, int64_t max_n
  *   gives zeros and takes no gradient.
  * n_b = key_lengths[b] (device, clamped to 0 .. Lk) or Lk where key_lengths is NULL; k and v behind it are not used, whatever they hold.
  * *_strides: HOST arrays of three element strides (sequence, token, head); the last dimension is contiguous.  Pointers and strides are
- * multiples of 16 bytes (COIN_EALIGN), strides may be 0; 130 tokens' span below 2^31 bytes, D <= 128 and a multiple of 8 (bf16) / 4 (f32)
- * (COIN_ESHAPE); 0 < scale <= 1e30.
+ * multiples of 16 bytes (COIN_EALIGN), strides may be 0; 130 tokens and the Hq / Hkv heads of a group within 2^31 bytes, D <= 128 and a
+ * multiple of 8 (bf16) / 4 (f32) (COIN_ESHAPE); 0 < scale <= 1e30.
  * lse (float32 [B][Hkv][Lq * Hq / Hkv], or NULL when no backward follows): log2 of the row's sum of exp, +inf without a key.
  * out_lo (bfloat16, contiguous like out, 16-byte aligned, or NULL when no backward follows; not used in float32): what rounding took from out.
  * workspace: coin_attention_workspace_bytes (0: none), 16-byte aligned. */
@@ -489,9 +489,10 @@ int coin_attention_bwd(const void* q, const int64_t* q_strides, const void* k, c
 /* Residual add with the norm behind the branch, its gate and scale, and the norm before the next branch:
  *   r = x + scale * gate o N_post(y),   h = N_pre(r),    N = LayerNorm, or RMSNorm where rms != 0
  * x, r [M][D] of stream_dtype; y, h [M][D] of branch_dtype (float32 streams take both types of branch, bfloat16 streams bfloat16); gate
- * [M / rows_per_gate][D] of gate_dtype, or NULL; weights and biases float32 [D] or NULL (1 and 0).  y NULL: h = N_pre(x), r is not
- * written.  has_post / has_pre: which norms there are.  Contiguous rows, D <= 8192 (COIN_ESHAPE); any D and alignment (rows of 16-byte
- * chunks are the fast ones).  stats float32 [M][4], 16-byte aligned, or NULL when no backward follows. */
+ * [M / rows_per_gate][D] of gate_dtype, or NULL; rows_per_gate divides M, also where gate is NULL (1 will do); weights and biases float32
+ * [D] or NULL (1 and 0).  y NULL: h = N_pre(x), r is not written.  has_post / has_pre: which norms there are.  Contiguous rows, D <= 8192
+ * (COIN_ESHAPE); any D and alignment (rows of 16-byte chunks are the fast ones).  stats float32 [M][4], 16-byte aligned, or NULL when no
+ * backward follows. */
 int coin_residual_norm_fwd(const void* x, const void* y, const void* gate, int64_t rows_per_gate, const float* post_weight, const float* post_bias,
                            int has_post, float post_eps, const float* pre_weight, const float* pre_bias, int has_pre, float pre_eps, int rms,
                            float scale, void* r, void* h, float* stats, int64_t M, int D, int stream_dtype, int branch_dtype, int gate_dtype,
