@@ -1024,7 +1024,7 @@ def chunked_heads(t: torch.Tensor, group: int = 1) -> torch.Tensor:
 class AttentionPlan:
     """What an attention call's shapes, strides and type decide: checked sizes, the strides of its eight tensors as the C ABI takes them (out
     and the gradients contiguous, or the gradients strided like one [B, L, 3, H, D] tensor), workspace sizes."""
-    __slots__ = ("dims", "group", "code", "strides", "at", "ws_fwd", "ws_bwd", "out_shape", "out_stride", "k_shape")
+    __slots__ = ("dims", "group", "packed", "layout", "code", "strides", "at", "ws_fwd", "ws_bwd", "out_shape", "out_stride", "k_shape")
 
     def __init__(self, q, k, v, packed: bool):
         if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
@@ -1038,7 +1038,7 @@ class AttentionPlan:
             raise CoinHipError(f"attention: {hq} query heads over {hkv} key heads")
         if d > 128 or d <= 0 or d % (16 // q.element_size()):
             raise CoinHipError(f"attention: head dimension {d} (a multiple of {16 // q.element_size()}, at most 128, for {q.dtype})")
-        self.dims, self.group = (b, lq, lk, hq, hkv, d), hq // hkv
+        self.dims, self.group, self.packed, self.layout = (b, lq, lk, hq, hkv, d), hq // hkv, packed, (q.stride(), k.stride(), v.stride())
         self.out_shape, self.k_shape, self.out_stride = tuple(q.shape), tuple(k.shape), (lq * hq * d, hq * d, d, 1)
         whole = [lq * hq * d, hq * d, d]
         grads = [[3 * lq * hq * d, 3 * hq * d, d]] * 3 if packed else [whole] + [[lk * hkv * d, hkv * d, d]] * 2
@@ -1062,6 +1062,15 @@ def attention_plan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packed: bo
             _ATTN_PLANS.clear()
         _ATTN_PLANS[key] = plan
     return plan
+
+
+def attention_saved(plan: AttentionPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
+    """-> (plan, q, k, v) for operands that come back from autograd: as they are, unless a saved-tensor hook (an offload to the host, a copy) laid them
+    out anew -- the plan's strides would reach outside them."""
+    if (q.stride(), k.stride(), v.stride()) == plan.layout:
+        return plan, q, k, v
+    q, k, v = chunked_heads(q, plan.group), chunked_heads(k), chunked_heads(v)
+    return attention_plan(q, k, v, plan.packed), q, k, v
 
 
 def attention_fwd(plan: AttentionPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scale: float,

@@ -921,7 +921,8 @@ class _Attention(Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lo, lse, lengths = ctx.saved_tensors
-        plan, dt, dev = ctx.plan, q.dtype, q.device
+        plan, q, k, v = K.attention_saved(ctx.plan, q, k, v)
+        dt, dev = q.dtype, q.device
         dq, dk, dv = (torch.empty(s, dtype=dt, device=dev) for s in (plan.out_shape, plan.k_shape, plan.k_shape))
         K.attention_bwd(plan, q, k, v, out, lo, K.chunked_heads(dout, plan.group), lse, ctx.causal, ctx.scale, lengths, dq, dk, dv)
         return dq, dk, dv, None, None, None, None
@@ -943,7 +944,8 @@ class _AttentionQKV(Function):
     def backward(ctx, dout):
         qkv, out, lo, lse, lengths = ctx.saved_tensors
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        K.attention_bwd(ctx.plan, *qkv.unbind(2), out, lo, K.chunked_heads(dout), lse, ctx.causal, ctx.scale, lengths, *dqkv.unbind(2))
+        plan, q, k, v = K.attention_saved(ctx.plan, *qkv.unbind(2))
+        K.attention_bwd(plan, q, k, v, out, lo, K.chunked_heads(dout), lse, ctx.causal, ctx.scale, lengths, *dqkv.unbind(2))
         return dqkv, None, None, None, None
 
 

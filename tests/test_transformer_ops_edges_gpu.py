@@ -284,3 +284,39 @@ def test_queries_that_see_no_key_may_hold_anything(shape, dtype):
         within(bad, *ref[name], name)
         if name in ("out", "dq"):
             assert not bad[dead].any(), name
+
+
+# ------------------------------------------------------------------------------------------------------- operands kept elsewhere meanwhile
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("keep", ["copies", "host"])
+def test_operands_that_a_saved_tensor_hook_lays_out_anew(keep, dtype):
+    """Copies and the host's offload give strided operands back dense: the gradients are those without a hook."""
+    hook = lambda: (torch.autograd.graph.save_on_cpu() if keep == "host"  # noqa: E731
+                    else torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t))
+    base = rand((3, 40, 3, 4, 64), dtype, 1)
+    wide = rand((3, 40, 1024), dtype, 2)[..., 128:896]
+    x, w = rand((50, 200), dtype, 3)[:, 8:72], rand((96, 128), dtype, 4, 0.1)[:, 64:]
+    ln = torch.nn.LayerNorm(64, device=DEV)
+
+    def views(t):
+        return L.attention(*t.unbind(2), causal=True, key_lengths=n)
+
+    def packed(t):
+        return L.attention_qkv(t, 4, causal=True)
+
+    def linear(t):
+        return L.fused_linear(t, w, act=L.ACT_GELU)
+
+    def norm(t):
+        return L.residual_norm(t, t.flip(0), post_norm=ln, pre_norm=ln)[1]
+
+    n = torch.tensor([40, 7, 33], device=DEV, dtype=torch.int32)
+    for f, src in ((views, base), (packed, wide), (linear, x), (norm, x)):
+        t = src.detach().requires_grad_()
+        assert f in (views,) or not t.is_contiguous()
+        with hook():
+            out = f(t)
+        dout = rand(out.shape, out.dtype, 9)
+        got, = torch.autograd.grad(out, t, dout)
+        want, = torch.autograd.grad(f(t), t, dout)
+        assert torch.equal(got, want), f.__name__
